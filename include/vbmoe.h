@@ -37,13 +37,17 @@ typedef enum vbm_status {
     VBM_ERR_OUT_OF_MEMORY = 4
 } vbm_status;
 
-/* ggml type ids (ggml.h enum ggml_type; MXFP4 = 39 per tests/test_cpu_research.py:56). */
+/* ggml type ids (ggml.h enum ggml_type; MXFP4 = 39 per tests/test_cpu_research.py:56). ggml has no
+ * 8-bit floating-point type: F8_E4M3 (OCP e4m3: 4 exponent bits with bias 7, no infinities, NaN 0x7F /
+ * 0xFF, largest value 448) is this library's own id. */
 enum {
     VBM_TYPE_F32 = 0,
     VBM_TYPE_F16 = 1,
     VBM_TYPE_Q8_0 = 8,
     VBM_TYPE_I32 = 26,
-    VBM_TYPE_MXFP4 = 39
+    VBM_TYPE_BF16 = 30,
+    VBM_TYPE_MXFP4 = 39,
+    VBM_TYPE_F8_E4M3 = 256
 };
 
 /* Activation of the expert FFN (tools/engine/f32_experts.hpp:14 F32Activation). */
@@ -267,6 +271,66 @@ vbm_status vbm_group_by_expert(const int32_t * ids, int64_t n_ids, int64_t n_tok
  * y [rows, n_ids, n_tokens] and weights [n_ids, n_tokens]. */
 vbm_status vbm_weighted_combine(const float * y, const float * weights, int64_t rows,
                                 int64_t n_ids, int64_t n_tokens, float * out, void * stream);
+
+/* ----------------------------------------------------------------------------------------------
+ * Block-scaled FP8 and 16-bit products, for checkpoints whose weights are kept as they are stored:
+ * row-major matrices of e4m3 codes with one fp32 scale per 128 x 128 block, or of fp16 / bf16. No
+ * counterpart in the reference (its expert weights are ggml-quantized); they take the router's, the
+ * grouping's and the combine's buffers as the calls above leave them:
+ *
+ *   vbm_router_topk_softmax -> ids, weights
+ *   vbm_group_by_expert     -> offsets, rows
+ *   vbm_quantize_fp8        x -> codes, scales [n_tokens]
+ *   vbm_grouped_mul_mat     gate_up: b_rows = rows, b_div = top_k -> grouped rows [2 * I]
+ *   vbm_glu_quantize_fp8    gate | up halves -> codes, scales, grouped
+ *   vbm_grouped_mul_mat     down: dst_rows = rows -> y [n_tokens][top_k][H] (F32)
+ *   vbm_weighted_combine    y, weights -> out [n_tokens][H]
+ *
+ * None of them allocates, needs a workspace or waits: all can be captured in a HIP graph, and calls on
+ * different streams do not share anything. Buffers belong to the current device. Results do not depend on
+ * what else runs, and a call repeated on the same inputs gives the same bits.
+ * -------------------------------------------------------------------------------------------- */
+/* Rows of x (F32, F16 or BF16; row stride x_stride elements) -> e4m3 codes [n_rows][k] (16-byte aligned) and
+ * fp32 scales [n_rows][ceil(k / 128)]; k a multiple of 16. For a run of 128 values (the last one of a row
+ * may be shorter) with a = max(max |x|, 2^-116): scale = a / 448, code = e4m3(448 x / a), the quotient
+ * correctly rounded in fp32 and then to the nearest e4m3 value, ties to even. A run that holds a NaN or an
+ * infinity gets the scale NaN and zero codes. n_rows = 0 does nothing. */
+vbm_status vbm_quantize_fp8(int x_type, const void * x, int64_t n_rows, int64_t k, int64_t x_stride, void * codes,
+                            float * scales, void * stream);
+/* act(gate, up) of vbm_glu (activation, alpha, limit as there) in fp32, quantized as by vbm_quantize_fp8:
+ * gate and up rows of `width` values of x_type with their own strides (the halves of a fused gate_up row:
+ * up = gate + width, both strides 2 * width). */
+vbm_status vbm_glu_quantize_fp8(int activation, int x_type, const void * gate, const void * up, int64_t n_rows,
+                                int64_t width, int64_t gate_stride, int64_t up_stride, float alpha, float limit,
+                                void * codes, float * scales, void * stream);
+
+/* n_groups weight matrices [rows][k], one after the other (device memory, 16-byte aligned). */
+typedef struct vbm_weights {
+    int type;                      /* VBM_TYPE_F8_E4M3 (k % 16 == 0), VBM_TYPE_F16 or VBM_TYPE_BF16 (k % 8 == 0) */
+    const void * data;             /* [n_groups][rows][k]                                        */
+    const float * scales;          /* F8: [n_groups][ceil(rows / 128)][ceil(k / 128)], else unused */
+    const float * bias;            /* [n_groups][rows] or NULL                                   */
+    int64_t n_groups;              /* 1..1024                                                    */
+    int64_t rows, k;
+} vbm_weights;
+
+/* dst[t][n] = w[n] . b[t] (+ bias[n]) of one FP8 matrix with tokens quantized by vbm_quantize_fp8: b codes
+ * [n_tokens][k] (16-byte aligned), b_scales [n_tokens][ceil(k / 128)], dst [n_tokens][rows] of dst_type (F32, F16 or
+ * BF16). Every sum is fp32 and rounded to dst_type once. n_tokens = 0 does nothing. */
+vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type,
+                           void * dst, void * stream);
+
+/* The products of rows grouped by expert, with any number of rows a group: for every group g and i in
+ * [offsets[g], offsets[g + 1]),
+ *   dst[dst_rows ? dst_rows[i] : i] = w[g] . b[b_rows ? b_rows[i] / b_div : i] (+ bias[g])
+ * offsets [n_groups + 1] as vbm_group_by_expert writes them, n_rows >= offsets[n_groups] the most rows there
+ * can be (its n_ids * n_tokens); neither is read on the host. b is [n_b][k] in the weights' type (F8: codes with
+ * b_scales [n_b][ceil(k / 128)]), dst [n_dst][rows] of dst_type. A b row outside [0, n_b) makes its outputs NaN; a dst
+ * row outside [0, n_dst) is not written, nor are dst rows that no group lists. dst_rows must not list a
+ * row twice. n_rows = 0 does nothing. */
+vbm_status vbm_grouped_mul_mat(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_b,
+                               const int32_t * b_rows, int64_t b_div, const int32_t * offsets, int64_t n_rows,
+                               const int32_t * dst_rows, int64_t n_dst, int dst_type, void * dst, void * stream);
 
 /* ----------------------------------------------------------------------------------------------
  * Fused routed-expert layer (expert_branch of hybrid-experts.patch:1394-1683 for one layer:

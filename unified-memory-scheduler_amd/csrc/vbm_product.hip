@@ -1,0 +1,403 @@
+// Products of weight matrices with token rows, dense or grouped by expert: FP8 (e4m3) weights with one fp32 scale per
+// 128 x 128 block and activations with one per 128 values of a row, or fp16 / bf16 weights and activations.
+//
+//   FP8:    dst[t][n] = sum over blocks kb of ws[n / 128][kb] * bs[t][kb] * (sum over the block's k of w[n][k] b[t][k])
+//   16-bit: dst[t][n] = sum over k of w[n][k] b[t][k]
+//
+// plus a bias. Everything is laid out along k, so the kernels see rows of bytes and take 128 of them a step: one FP8 scale
+// block, or 64 16-bit values. As a matrix operand lane (q, r) = (lane / 16, lane % 16) holds 32 of row r's 128 bytes; which ones
+// does not matter as long as both operands agree. The weights are the A operand and the tokens B, so that a lane's four results
+// are four neighbouring outputs of one token.
+#include <algorithm>
+#include <type_traits>
+
+#include "vbm_device.hpp"
+#include "vbm_internal.hpp"
+
+namespace vbm {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4p __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2p __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_p __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_p __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_p __attribute__((ext_vector_type(8)));
+
+// How a step's 128 bytes a row are multiplied.
+//   kF8Wide: the e4m3 codes widened to fp16 (exact) and multiplied as such: exact products, fp32 sums.
+//   kF16, kBF16: as they are.
+enum Kind { kF8Wide, kF16, kBF16 };
+constexpr bool is_f8(int kind) { return kind == kF8Wide; }
+
+struct ProductArgs {
+    const uint8_t * w;             // [n_groups][rows][k_bytes]
+    const float * ws;              // [n_groups][ceil(rows / 128)][kb], FP8 only
+    const float * bias;            // [n_groups][rows] or null
+    const uint8_t * b;             // [n_b][k_bytes]
+    const float * bs;              // [n_b][kb], FP8 only
+    int64_t n_b;
+    const int32_t * b_rows;        // grouped row -> b row times b_div, or null (b row = grouped row)
+    int64_t b_div;
+    const int32_t * offsets;       // [n_groups + 1] or null (one group of n_rows)
+    int64_t n_rows;
+    const int32_t * dst_rows;      // grouped row -> dst row, or null
+    int64_t n_dst;
+    void * dst;
+    int dst_type, dst_vec;         // dst_vec: four neighbouring outputs can be stored at once
+    int n_groups, rows, k_bytes, kb;
+};
+
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row 0's last to row 1, row 2's to row 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // lane 31's to the upper half
+    return v;
+}
+
+struct TokenTile {
+    int group;
+    int64_t first, last;           // grouped rows [first, last)
+};
+
+// The group and rows of token tile `index`, tiles of BT rows in group order; false past the last one. Every wave finds it
+// from the offsets by itself (the host does not know the groups' sizes, and a launch that wrote the list would cost more). Offsets
+// are bounded to [0, n_rows], so that bad ones cannot lead out of the buffers.
+__device__ __forceinline__ bool find_token_tile(const ProductArgs & A, int index, int tile_rows, TokenTile & t) {
+    if (!A.offsets) {
+        t.group = 0;
+        t.first = static_cast<int64_t>(index) * tile_rows;
+        t.last = t.first + tile_rows < A.n_rows ? t.first + tile_rows : A.n_rows;
+        return t.first < A.n_rows;
+    }
+    const int lane = threadIdx.x & 63;
+    const int n_rows = static_cast<int>(A.n_rows);
+    auto bounded = [&](int v) { return v < 0 ? 0 : (v > n_rows ? n_rows : v); };
+    int before = 0;
+    for (int g0 = 0; g0 < A.n_groups; g0 += 64) {
+        const int g = g0 + lane;
+        const bool live = g < A.n_groups;
+        const int lo = live ? bounded(A.offsets[g]) : 0, hi = live ? bounded(A.offsets[g + 1]) : 0;
+        const int tiles = hi > lo ? (hi - lo + tile_rows - 1) / tile_rows : 0;
+        const int incl = before + wave_inclusive_sum(tiles);
+        const uint64_t past = __ballot(incl > index);
+        if (past) {
+            const int who = __builtin_ctzll(past);
+            const int start = __shfl(lo, who) + (index - __shfl(incl - tiles, who)) * tile_rows, end = __shfl(hi, who);
+            t.group = __builtin_amdgcn_readfirstlane(g0 + who);
+            t.first = __builtin_amdgcn_readfirstlane(start);
+            t.last = __builtin_amdgcn_readfirstlane(start + tile_rows < end ? start + tile_rows : end);
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+}
+
+// Grouped row i's row of b; -1: none (its outputs are NaN).
+__device__ __forceinline__ int64_t source_row(const ProductArgs & A, int64_t i) {
+    if (!A.b_rows) return i < A.n_b ? i : -1;
+    const int64_t v = A.b_rows[i];
+    if (v < 0) return -1;
+    const int64_t row = static_cast<uint32_t>(v) / static_cast<uint32_t>(A.b_div);
+    return row < A.n_b ? row : -1;
+}
+// Its place in dst; -1: not written.
+__device__ __forceinline__ int64_t target_row(const ProductArgs & A, int64_t i) {
+    const int64_t row = A.dst_rows ? A.dst_rows[i] : i;
+    return row >= 0 && row < A.n_dst ? row : -1;
+}
+
+// A lane's 32 bytes of a step.
+struct Piece {
+    u32x4p lo, hi;
+};
+
+__device__ __forceinline__ uint16_t to_bf16(float v) {   // nearest even; NaN stays NaN
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    if (v != v) return 0x7FC0;
+    return static_cast<uint16_t>((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ uint16_t to_16(int type, float v) {
+    return type == VBM_TYPE_BF16 ? to_bf16(v) : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+}
+
+// Outputs n .. n + 3 of one dst row.
+__device__ __forceinline__ void store4(const ProductArgs & A, int64_t row, int n, f32x4 v) {
+    const int64_t at = row * A.rows + n;
+    if (A.dst_type == VBM_TYPE_F32) {
+        float * p = static_cast<float *>(A.dst) + at;
+        if (A.dst_vec && n + 4 <= A.rows) {
+            *reinterpret_cast<f32x4 *>(p) = v;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < A.rows) p[i] = v[i];
+        return;
+    }
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = to_16(A.dst_type, v[i]);
+    uint16_t * p = static_cast<uint16_t *>(A.dst) + at;
+    if (A.dst_vec && n + 4 <= A.rows) {
+        *reinterpret_cast<u32x2p *>(p) = u32x2p{h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < A.rows) p[i] = h[i];
+}
+
+__device__ __forceinline__ half8_p widened(unsigned a, unsigned b) {
+    const half2_p p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+    const half2_p p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+    return half8_p{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+}
+
+// A piece as matrix operands, and the product of two of them added to c.
+template <int KIND>
+struct Operand {
+    static constexpr int N = is_f8(KIND) ? 4 : 2;
+    using T = std::conditional_t<KIND == kBF16, bf16x8_p, half8_p>;
+    T v[N];
+    __device__ __forceinline__ void take(const Piece & p) {
+        if constexpr (is_f8(KIND)) {
+            v[0] = widened(p.lo.x, p.lo.y), v[1] = widened(p.lo.z, p.lo.w);
+            v[2] = widened(p.hi.x, p.hi.y), v[3] = widened(p.hi.z, p.hi.w);
+        } else {
+            v[0] = __builtin_bit_cast(T, p.lo), v[1] = __builtin_bit_cast(T, p.hi);
+        }
+    }
+};
+template <int KIND>
+__device__ __forceinline__ f32x4 product(const Operand<KIND> & a, const Operand<KIND> & b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < Operand<KIND>::N; ++i) {
+        if constexpr (KIND == kBF16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+        else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[i], b.v[i], c, 0, 0, 0);
+    }
+    return c;
+}
+
+// ------------------------------------------------------------------------------- few tokens a group
+// A workgroup takes 16 * RS weight rows x up to 16 * NT tokens of one group; its W waves share the depth and add their sums up
+// through LDS, in wave order. Weights and tokens go from memory to registers: with few tokens a group the weights'
+// bytes are the work, and nobody else in the workgroup needs them.
+template <int KIND, int NT, int RS, int W>
+__global__ __launch_bounds__(W * 64) void few_rows_kernel(ProductArgs A, int row_tiles) {
+    constexpr int U = NT * RS <= 2 ? 4 : 2;                  // steps whose loads go out together
+    __shared__ f32x4 parts[W][RS * NT][64];
+    TokenTile t;
+    const int token_tile = static_cast<int>(blockIdx.x) / row_tiles, n0 = (static_cast<int>(blockIdx.x) - token_tile * row_tiles) * (16 * RS);
+    if (!find_token_tile(A, token_tile, 16 * NT, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int q = lane >> 4, r = lane & 15;
+
+    // lane (q, r) brings 16-byte pieces q and q + 4 of a step: the four lanes of a row read 64 bytes side by side
+    const uint8_t * wp[RS], * bp[NT];
+    const float * bsp[NT], * wsp = nullptr;
+    bool bad[NT];
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        const int row = n0 + 16 * s + r < A.rows ? n0 + 16 * s + r : A.rows - 1;
+        wp[s] = A.w + (static_cast<int64_t>(t.group) * A.rows + row) * A.k_bytes + q * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t i = t.first + 16 * j + r;
+        const int64_t src = source_row(A, i < t.last ? i : t.first);   // (spare columns repeat the tile's first token)
+        bad[j] = src < 0;
+        bp[j] = A.b + (bad[j] ? 0 : src) * A.k_bytes + q * 16;
+        if constexpr (is_f8(KIND)) bsp[j] = A.bs + (bad[j] ? 0 : src) * A.kb;
+    }
+    if constexpr (is_f8(KIND)) wsp = A.ws + (static_cast<int64_t>(t.group) * ((A.rows + 127) >> 7) + (n0 >> 7)) * A.kb;
+
+    f32x4 acc[RS][NT];
+#pragma unroll
+    for (int s = 0; s < RS; ++s)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // UU steps from kb on; TAIL: the row's last step, whose pieces past the row are zeros
+    auto steps = [&](auto uu_c, auto tail_c, int kb) __attribute__((always_inline)) {
+        constexpr int UU = decltype(uu_c)::value;
+        constexpr bool TAIL = decltype(tail_c)::value;
+        const int left = A.k_bytes - kb * 128 - q * 16;       // bytes of the row from this lane's first piece on
+        auto piece = [&](const uint8_t * p, int u) __attribute__((always_inline)) {
+            const uint8_t * at = p + static_cast<int64_t>(kb + u) * 128;
+            Piece v{};
+            if (!TAIL || left > 0) v.lo = *reinterpret_cast<const u32x4p *>(at);
+            if (!TAIL || left > 64) v.hi = *reinterpret_cast<const u32x4p *>(at + 64);
+            return v;
+        };
+        Piece wv[UU][RS], bv[UU][NT];
+        float sc[UU][NT], sw[UU];
+#pragma unroll
+        for (int u = 0; u < UU; ++u) {
+#pragma unroll
+            for (int s = 0; s < RS; ++s) wv[u][s] = piece(wp[s], u);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) bv[u][j] = piece(bp[j], u);
+            if constexpr (is_f8(KIND)) {
+                sw[u] = wsp[kb + u];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) sc[u][j] = bsp[j][kb + u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UU; ++u) {
+            Operand<KIND> a[RS];
+#pragma unroll
+            for (int s = 0; s < RS; ++s) a[s].take(wv[u][s]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                Operand<KIND> b;
+                b.take(bv[u][j]);
+#pragma unroll
+                for (int s = 0; s < RS; ++s) {
+                    if constexpr (is_f8(KIND)) {
+                        const f32x4 p = product<KIND>(a[s], b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        const float f = sw[u] * sc[u][j];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[s][j][i] = __builtin_fmaf(p[i], f, acc[s][j][i]);
+                    } else {
+                        acc[s][j] = product<KIND>(a[s], b, acc[s][j]);
+                    }
+                }
+            }
+        }
+    };
+    using One = std::integral_constant<int, 1>;
+    const int k_end = A.kb * (wave + 1) / W, whole = A.k_bytes >> 7;
+    int kb = A.kb * wave / W;
+    for (; kb + U <= (k_end < whole ? k_end : whole); kb += U) steps(std::integral_constant<int, U>{}, std::false_type{}, kb);
+    for (; kb < (k_end < whole ? k_end : whole); ++kb) steps(One{}, std::false_type{}, kb);
+    if (kb < k_end) steps(One{}, std::true_type{}, kb);
+
+#pragma unroll
+    for (int s = 0; s < RS; ++s)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) parts[wave][s * NT + j][lane] = acc[s][j];
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < RS * NT; ++f) {
+        if (f % W != wave) continue;
+        const int s = f / NT, j = f % NT;
+        f32x4 v = parts[0][f][lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v += parts[w][f][lane];
+        const int n = n0 + 16 * s + 4 * q;
+        const int64_t i = t.first + 16 * j + r;
+        if (i >= t.last || n >= A.rows) continue;
+        const int64_t row = target_row(A, i);
+        if (row < 0) continue;
+        if (A.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(t.group) * A.rows + n + e];
+        }
+        const float nan = __builtin_nanf("");
+        store4(A, row, n, bad[j] ? f32x4{nan, nan, nan, nan} : v);
+    }
+}
+
+// Most token tiles of `tile_rows` that n_rows rows in n_groups groups can have.
+int64_t most_token_tiles(const ProductArgs & a, int tile_rows) {
+    const int64_t whole = (a.n_rows + tile_rows - 1) / tile_rows;
+    return a.offsets ? std::min(a.n_rows, a.n_rows / tile_rows + a.n_groups) : whole;
+}
+
+template <int KIND, int NT, int RS, int W>
+void launch_few_rows(const ProductArgs & a, hipStream_t stream) {
+    const int64_t row_tiles = (a.rows + 16 * RS - 1) / (16 * RS), blocks = row_tiles * most_token_tiles(a, 16 * NT);
+    require(blocks < (int64_t{1} << 32) / (W * 64), "too many outputs for one launch");
+    hipLaunchKernelGGL((few_rows_kernel<KIND, NT, RS, W>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, stream, a,
+                       static_cast<int>(row_tiles));
+    check_hip(hipGetLastError(), "product launch");
+}
+
+template <int KIND>
+void launch_product(const ProductArgs & a, hipStream_t stream) {
+    if (a.n_rows == 0 || a.rows == 0) return;
+    const int64_t mean = a.n_rows / std::min<int64_t>(a.n_groups, a.n_rows);
+    if (mean <= 16) launch_few_rows<KIND, 1, 1, 4>(a, stream);
+    else launch_few_rows<KIND, 4, 2, 4>(a, stream);
+}
+
+void product(const vbm_weights & w, const void * b, const float * b_scales, ProductArgs a, int dst_type, void * dst, hipStream_t stream) {
+    const bool f8 = w.type == VBM_TYPE_F8_E4M3;
+    require(f8 || w.type == VBM_TYPE_F16 || w.type == VBM_TYPE_BF16, "weights must be F8_E4M3, F16 or BF16");
+    require(dst_type == VBM_TYPE_F32 || dst_type == VBM_TYPE_F16 || dst_type == VBM_TYPE_BF16, "dst must be F32, F16 or BF16");
+    require(w.n_groups > 0 && w.n_groups <= 1024, "n_groups must be in 1..1024");
+    require(w.rows > 0 && w.rows < (int64_t{1} << 30) && w.k > 0 && w.k < (int64_t{1} << 29), "rows and k out of range");
+    const int64_t k_bytes = w.k * (f8 ? 1 : 2);
+    require(k_bytes % 16 == 0, f8 ? "k must be a multiple of 16" : "k must be a multiple of 8");
+    require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 31) && a.n_b >= 0 && a.n_dst >= 0, "row counts out of range");
+    require(a.b_div > 0 && a.b_div < (int64_t{1} << 31), "b_div must be positive");
+    if (a.n_rows == 0) return;
+    require(w.data && b && dst && a.n_b > 0 && (!f8 || (w.scales && b_scales)), "null buffer");
+    auto at = [](const void * p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+    require(at(w.data, 16) && at(b, 16), "weights and b must be 16-byte aligned");
+    const size_t dsize = dst_type == VBM_TYPE_F32 ? 4 : 2;
+    require(at(dst, dsize) && at(w.scales, 4) && at(w.bias, 4) && at(b_scales, 4) && at(a.offsets, 4) && at(a.b_rows, 4) && at(a.dst_rows, 4),
+            "buffers must be aligned to their types");
+    a.w = static_cast<const uint8_t *>(w.data);
+    a.ws = w.scales;
+    a.bias = w.bias;
+    a.b = static_cast<const uint8_t *>(b);
+    a.bs = b_scales;
+    a.dst = dst;
+    a.dst_type = dst_type;
+    a.dst_vec = at(dst, 4 * dsize) && w.rows % 4 == 0;
+    a.n_groups = static_cast<int>(w.n_groups);
+    a.rows = static_cast<int>(w.rows);
+    a.k_bytes = static_cast<int>(k_bytes);
+    a.kb = static_cast<int>((k_bytes + 127) / 128);
+    if (f8) launch_product<kF8Wide>(a, stream);
+    else if (w.type == VBM_TYPE_F16) launch_product<kF16>(a, stream);
+    else launch_product<kBF16>(a, stream);
+}
+
+}  // namespace
+}  // namespace vbm
+
+using namespace vbm;
+
+extern "C" {
+
+vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type,
+                           void * dst, void * stream) {
+    return guarded([&] {
+        require(w != nullptr, "null weights");
+        require(w->type == VBM_TYPE_F8_E4M3 && w->n_groups == 1, "weights must be one F8_E4M3 matrix");
+        ProductArgs a{};
+        a.n_b = a.n_rows = a.n_dst = n_tokens;
+        a.b_div = 1;
+        product(*w, b, b_scales, a, dst_type, dst, as_stream(stream));
+    });
+}
+
+vbm_status vbm_grouped_mul_mat(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_b,
+                               const int32_t * b_rows, int64_t b_div, const int32_t * offsets, int64_t n_rows,
+                               const int32_t * dst_rows, int64_t n_dst, int dst_type, void * dst, void * stream) {
+    return guarded([&] {
+        require(w != nullptr, "null weights");
+        require(offsets != nullptr || n_rows == 0, "null offsets");
+        ProductArgs a{};
+        a.n_b = n_b;
+        a.b_rows = b_rows;
+        a.b_div = b_div;
+        a.offsets = offsets;
+        a.n_rows = n_rows;
+        a.dst_rows = dst_rows;
+        a.n_dst = n_dst;
+        product(*w, b, b_scales, a, dst_type, dst, as_stream(stream));
+    });
+}
+
+}  // extern "C"

@@ -15,7 +15,7 @@ import numpy as np
 LIB_PATH = Path(__file__).resolve().parent / "libvbmoe.so"
 HEADER = Path(__file__).resolve().parents[2] / "include" / "vbmoe.h"
 
-TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_I32, TYPE_MXFP4 = 0, 1, 8, 26, 39
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_I32, TYPE_BF16, TYPE_MXFP4, TYPE_F8_E4M3 = 0, 1, 8, 26, 30, 39, 256
 ACT_SILU, ACT_SWIGLU_OAI = 0, 1
 ORDER_EXACT, ORDER_FAST = 0, 1
 STATUS = {0: "OK", 1: "INVALID_ARGUMENT", 2: "RUNTIME", 3: "UNSUPPORTED", 4: "OUT_OF_MEMORY"}
@@ -118,6 +118,11 @@ class MoeLayerDesc(C.Structure):
     ]
 
 
+class Weights(C.Structure):
+    """vbm_weights: n_groups row-major matrices [rows][k] of F8_E4M3 (with block scales), F16 or BF16."""
+    _fields_ = [("type", C.c_int), ("data", vp), ("scales", vp), ("bias", vp), ("n_groups", i64), ("rows", i64), ("k", i64)]
+
+
 # name -> argtypes (all return vbm_status as c_int)
 SIGNATURES = {
     "vbm_device_count": [C.POINTER(C.c_int)],
@@ -166,6 +171,10 @@ SIGNATURES = {
     "vbm_router_topk_softmax": [vp, vp, vp, i64, vp, i64, i64, i64, vp, vp, vp],
     "vbm_group_by_expert": [vp, i64, i64, i64, i64, vp, vp, vp, vp, vp],
     "vbm_weighted_combine": [vp, vp, i64, i64, i64, vp, vp],
+    "vbm_quantize_fp8": [C.c_int, vp, i64, i64, i64, vp, vp, vp],
+    "vbm_glu_quantize_fp8": [C.c_int, C.c_int, vp, vp, i64, i64, i64, i64, C.c_float, C.c_float, vp, vp, vp],
+    "vbm_mul_mat_fp8": [C.POINTER(Weights), vp, vp, i64, C.c_int, vp, vp],
+    "vbm_grouped_mul_mat": [C.POINTER(Weights), vp, vp, i64, vp, i64, vp, i64, vp, i64, C.c_int, vp, vp],
     "vbm_moe_layer_workspace": [C.POINTER(MoeLayerDesc), i64, C.POINTER(sz)],
     "vbm_moe_layer_forward": [C.POINTER(MoeLayerDesc), vp, vp, i64, vp, vp, vp, vp, sz, vp],
     "vbm_moe_layer_forward_profiled": [C.POINTER(MoeLayerDesc), vp, vp, i64, vp, vp, vp, vp, sz, vp, vp],
