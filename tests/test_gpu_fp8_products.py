@@ -137,7 +137,7 @@ def test_glu_quantize_marks_blocks_without_a_scale(gpu):
 @pytest.mark.parametrize("dst_type", TYPES)
 @pytest.mark.parametrize("tokens,rows,k,bias", [(1, 64, 128, False), (1, 300, 2880, True), (2, 1, 16, True), (15, 129, 48, False), (16, 15, 144, False),
                                                 (17, 100, 336, True), (40, 130, 2048, False), (65, 257, 720, True), (130, 515, 400, False),
-                                                (300, 384, 1040, True)])
+                                                (300, 384, 1040, True), (2085, 6164, 144, True), (1000, 2000, 272, False)])
 def test_dense_product(gpu, dst_type, tokens, rows, k, bias):
     rng = np.random.default_rng(tokens * 31 + rows)
     m, x = R.Matrix(F8, rng, 1, rows, k, bias), R.Tokens(F8, rng, tokens, k)
@@ -193,6 +193,23 @@ def test_grouped_product_over_many_groups(gpu, type_id, groups):
     m, x = R.Matrix(type_id, rng, groups, 33, 128), R.Tokens(type_id, rng, used, 128)
     got = R.grouped(m, x, used, offsets, used, F32, used)
     R.check(m, F32, got, *R.grouped_want(m, x, used, offsets, used, used), f"{groups} groups")
+
+
+@pytest.mark.parametrize("type_id,dst_type", [(F8, F32), (F8, F16), (F8, BF16), (F16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("rows,k,groups,most", [(2100, 272, 24, 290), (1090, 400, 24, 290), (520, 656, 6, 290), (257, 1168, 3, 700)])
+def test_grouped_product_many_rows(gpu, type_id, dst_type, gather, rows, k, groups, most):
+    """Sizes from a few rows to several tiles a group, in launches that fill the card and small ones."""
+    rng = np.random.default_rng(rows + k + gather)
+    counts = np.concatenate([[0, 1, 2 * most // 3], rng.integers(0, most, groups)])[:groups]
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    n_rows, top_k = int(offsets[-1]) + 5, 3
+    place = rng.permutation(n_rows).astype(np.int32)
+    n_b = -(-n_rows // top_k) if gather else n_rows
+    m, x = R.Matrix(type_id, rng, groups, rows, k, bias=not gather), R.Tokens(type_id, rng, n_b, k)
+    kw = dict(b_rows=place, b_div=top_k) if gather else dict(dst_rows=place)
+    got = R.grouped(m, x, n_b, offsets, n_rows, dst_type, n_rows, **kw)
+    R.check(m, dst_type, got, *R.grouped_want(m, x, n_b, offsets, n_rows, n_rows, **kw), f"many rows {rows}x{k}")
 
 
 @pytest.mark.parametrize("type_id", [F8, F16])

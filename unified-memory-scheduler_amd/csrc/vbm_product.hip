@@ -27,9 +27,13 @@ typedef __bf16 bf16x8_p __attribute__((ext_vector_type(8)));
 
 // How a step's 128 bytes a row are multiplied.
 //   kF8Wide: the e4m3 codes widened to fp16 (exact) and multiplied as such: exact products, fp32 sums.
+//   kF8: by the FP8 matrix instruction, at twice that rate. It adds eight neighbouring products at a time, aligned to the largest of
+//        them and cut off 13 bits below its leading one (found by probing it with two products of different size); between such
+//        eights it sums in fp32. That is at most 7 * 2^-13 of the largest of eight, and 1.4e-5 to 6e-5 of the result on random data: far
+//        below the rounding of a 16-bit output (2^-9 or 2^-12 on average), which is what it is used for, and too much for fp32 ones.
 //   kF16, kBF16: as they are.
-enum Kind { kF8Wide, kF16, kBF16 };
-constexpr bool is_f8(int kind) { return kind == kF8Wide; }
+enum Kind { kF8Wide, kF8, kF16, kBF16 };
+constexpr bool is_f8(int kind) { return kind == kF8Wide || kind == kF8; }
 
 struct ProductArgs {
     const uint8_t * w;             // [n_groups][rows][k_bytes]
@@ -162,11 +166,13 @@ __device__ __forceinline__ half8_p widened(unsigned a, unsigned b) {
 // A piece as matrix operands, and the product of two of them added to c.
 template <int KIND>
 struct Operand {
-    static constexpr int N = is_f8(KIND) ? 4 : 2;
-    using T = std::conditional_t<KIND == kBF16, bf16x8_p, half8_p>;
+    static constexpr int N = KIND == kF8 ? 1 : (KIND == kF8Wide ? 4 : 2);
+    using T = std::conditional_t<KIND == kF8, i32x8, std::conditional_t<KIND == kBF16, bf16x8_p, half8_p>>;
     T v[N];
     __device__ __forceinline__ void take(const Piece & p) {
-        if constexpr (is_f8(KIND)) {
+        if constexpr (KIND == kF8) {
+            v[0] = __builtin_bit_cast(i32x8, p);
+        } else if constexpr (KIND == kF8Wide) {
             v[0] = widened(p.lo.x, p.lo.y), v[1] = widened(p.lo.z, p.lo.w);
             v[2] = widened(p.hi.x, p.hi.y), v[3] = widened(p.hi.z, p.hi.w);
         } else {
@@ -178,7 +184,8 @@ template <int KIND>
 __device__ __forceinline__ f32x4 product(const Operand<KIND> & a, const Operand<KIND> & b, f32x4 c) {
 #pragma unroll
     for (int i = 0; i < Operand<KIND>::N; ++i) {
-        if constexpr (KIND == kBF16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+        if constexpr (KIND == kF8) c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v[i], b.v[i], c, 0, 0, 0, 0, 0, 0);
+        else if constexpr (KIND == kBF16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
         else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[i], b.v[i], c, 0, 0, 0);
     }
     return c;
@@ -306,6 +313,225 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(ProductArgs A, int row
     }
 }
 
+// ----------------------------------------------------------------------------------- many tokens
+// Tokens of a step and row's zero pieces past its end.
+__device__ const u32x4p zero_piece[1] = {};
+
+// Loads from memory to LDS (lane l's bytes land at m0 + l * size), in inline assembly so that the compiler does not wait for
+// all of them before every LDS read; the kernel waits itself before each barrier. The compiler knows of no other use of
+// M0 here, and the wait state between a scalar write of M0 and the load that reads it is written out.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_to_lds_16(const void * src, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// Waits until all but the wave's newest N loads have landed and its LDS reads are done, then for the workgroup's other waves.
+template <int N>
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+struct Work {
+    int group, row_tile;
+    int first, live;               // grouped rows
+};
+// The calling workgroup's share: a row tile x a token tile of at most `most` 16-token columns of one group. Workgroup i runs on XCD
+// i % 8, so each XCD takes a contiguous run of the list (group by group, row tile by row tile): the token tiles that share a row
+// tile's weights, and the row tiles that share the tokens, then meet in one L2. A group's tiles share its columns evenly.
+__device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int row_tiles, Work & w) {
+    const int lane = threadIdx.x & 63, n_rows = static_cast<int>(A.n_rows);
+    auto bounded = [&](int v) { return v < 0 ? 0 : (v > n_rows ? n_rows : v); };
+    auto columns = [&](int lo, int hi) { return hi > lo ? (hi - lo + 15) >> 4 : 0; };
+    auto tiles_of = [&](int cols) { return (cols + most - 1) / most; };
+    int total = 0;
+    if (!A.offsets) {
+        total = tiles_of(columns(0, n_rows));
+    } else {
+        int mine = 0;
+        for (int g = lane; g < A.n_groups; g += 64) mine += tiles_of(columns(bounded(A.offsets[g]), bounded(A.offsets[g + 1])));
+        total = __builtin_amdgcn_readlane(wave_inclusive_sum(mine), 63);
+    }
+    const int items = total * row_tiles, per_xcd = (items + 7) >> 3, slot = static_cast<int>(blockIdx.x >> 3);
+    const int item = static_cast<int>(blockIdx.x & 7) * per_xcd + slot;
+    if (slot >= per_xcd || item >= items) return false;
+    const int index = item / row_tiles;
+    int lo = 0, hi = n_rows, tiles = total, before = 0;
+    w.group = 0;
+    if (A.offsets) {
+        int sum = 0;
+        for (int g0 = 0; g0 < A.n_groups; g0 += 64) {
+            const int g = g0 + lane;
+            const int l = g < A.n_groups ? bounded(A.offsets[g]) : 0, h = g < A.n_groups ? bounded(A.offsets[g + 1]) : 0;
+            const int t = tiles_of(columns(l, h)), incl = sum + wave_inclusive_sum(t);
+            const uint64_t past = __ballot(incl > index);
+            if (past) {
+                const int who = __builtin_ctzll(past);
+                w.group = g0 + who;
+                lo = __builtin_amdgcn_readlane(l, who);
+                hi = __builtin_amdgcn_readlane(h, who);
+                tiles = __builtin_amdgcn_readlane(t, who);
+                before = __builtin_amdgcn_readlane(incl, who) - tiles;
+                break;
+            }
+            sum = __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+    const int local = item - before * row_tiles;
+    w.row_tile = local / tiles;
+    const int tile = local - w.row_tile * tiles, share = (columns(lo, hi) + tiles - 1) / tiles;
+    w.first = lo + tile * share * 16;
+    w.live = hi - w.first < share * 16 ? hi - w.first : share * 16;
+    return w.live > 0;
+}
+
+// A workgroup of WN x WT waves takes BN = 16 SN WN weight rows x up to BT = 16 ST WT tokens of one group; a wave 16 SN rows x every WT-th
+// 16-token column. A step's 128 bytes of every row are staged in LDS, STAGES - 1 steps ahead, with one wait and one barrier a
+// step. Piece p (16 bytes) of row r lies at place p ^ (r & 7) of the row's 128 bytes, so that sixteen rows' reads of one piece
+// spread over the banks.
+template <int KIND, int SN, int ST, int WN, int WT, int STAGES>
+__global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
+    constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
+    constexpr int DW = BN / 8 / W, DT = BT / 8 / W;          // a wave's loads a step: 8 rows each
+    static_assert(DW * 8 * W == BN && DT * 8 * W == BT && BT % 64 == 0, "the waves share the loads evenly");
+    constexpr int STAGE = (BN + BT) * 128 + (is_f8(KIND) ? BT * 4 : 0);
+    constexpr int PER_STEP = DW + DT + (is_f8(KIND) ? 1 : 0);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
+    Work work;
+    if (!find_work(A, ST * WT, row_tiles, work)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int q = lane >> 4, r = lane & 15, wn = wave / WT, wt = wave % WT;
+    const int n0 = work.row_tile * BN;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+
+    const uint8_t * wsrc[DW], * tsrc[DT];
+    const int piece = (lane & 7) ^ (lane >> 3);              // the one this lane brings of row lane / 8 of eight
+#pragma unroll
+    for (int i = 0; i < DW; ++i) {
+        const int n = n0 + 8 * (wave + W * i) + (lane >> 3);
+        wsrc[i] = A.w + (static_cast<int64_t>(work.group) * A.rows + (n < A.rows ? n : A.rows - 1)) * A.k_bytes + piece * 16;
+    }
+    auto token_row = [&](int i) __attribute__((always_inline)) {   // spare tokens repeat the first one, unknown ones read row 0
+        const int64_t src = source_row(A, work.first + (i < work.live ? i : 0));
+        return src < 0 ? 0 : src;
+    };
+#pragma unroll
+    for (int i = 0; i < DT; ++i) tsrc[i] = A.b + token_row(8 * (wave + W * i) + (lane >> 3)) * A.k_bytes + piece * 16;
+    const int scale_slot = wave % (BT / 64);
+    const float * ssrc = nullptr, * wscale = nullptr;
+    if constexpr (is_f8(KIND)) {
+        ssrc = A.bs + token_row(64 * scale_slot + lane) * A.kb;
+        const int block = (n0 + 16 * SN * wn) >> 7, last = (A.rows - 1) >> 7;
+        wscale = A.ws + (static_cast<int64_t>(work.group) * (last + 1) + (block < last ? block : last)) * A.kb;
+    }
+
+    const int live_cols = (work.live + 15) >> 4;
+    auto issue = [&](int kb) __attribute__((always_inline)) {
+        const uint32_t at = lds0 + (kb % STAGES) * STAGE;
+        const int k = kb < A.kb ? kb : A.kb - 1;             // (past the end: the last step again, into a stage that nobody reads)
+        const bool past = k * 128 + piece * 16 >= A.k_bytes;
+        auto from = [&](const uint8_t * p) __attribute__((always_inline)) {
+            return past ? reinterpret_cast<const uint8_t *>(zero_piece) : p + static_cast<int64_t>(k) * 128;
+        };
+#pragma unroll
+        for (int i = 0; i < DW; ++i) load_to_lds_16(from(wsrc[i]), at + (wave + W * i) * 1024);
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+            if (STAGES > 2 || 8 * (wave + W * i) < 16 * live_cols) load_to_lds_16(from(tsrc[i]), at + BN * 128 + (wave + W * i) * 1024);
+        if constexpr (is_f8(KIND)) load_to_lds_4(ssrc + k, at + (BN + BT) * 128 + scale_slot * 256);
+    };
+
+    auto run = [&](auto live_c) __attribute__((always_inline)) {
+        constexpr int NT = decltype(live_c)::value;
+        f32x4 acc[SN][NT];
+#pragma unroll
+        for (int s = 0; s < SN; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float scales = 0.0f;                                 // lane l: the weights' scale of step l (mod 64)
+        auto fetch_scales = [&](int kb) __attribute__((always_inline)) {
+            if constexpr (is_f8(KIND)) scales = kb + lane < A.kb ? wscale[kb + lane] : 0.0f;
+        };
+        fetch_scales(0);
+#pragma unroll
+        for (int kb = 0; kb < STAGES - 1; ++kb) issue(kb);
+        const int lo = r * 128 + ((2 * q) ^ (r & 7)) * 16, hi = r * 128 + ((2 * q + 1) ^ (r & 7)) * 16;
+        for (int kb = 0; kb < A.kb; ++kb) {
+            meet<(STAGES - 2) * PER_STEP>();
+            if (STAGES > 2 || kb + 1 < A.kb) issue(kb + STAGES - 1);
+            const uint8_t * stage = lds + (kb % STAGES) * STAGE;
+            auto operand = [&](int row) __attribute__((always_inline)) {
+                Operand<KIND> o;
+                o.take(Piece{*reinterpret_cast<const u32x4p *>(stage + row * 128 + lo), *reinterpret_cast<const u32x4p *>(stage + row * 128 + hi)});
+                return o;
+            };
+            Operand<KIND> a[SN];
+#pragma unroll
+            for (int s = 0; s < SN; ++s) a[s] = operand(16 * (SN * wn + s));
+            float sw = 0.0f;
+            if constexpr (is_f8(KIND)) {
+                if (kb && !(kb & 63)) fetch_scales(kb);
+                sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scales), kb & 63));
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int col = 16 * (j * WT + wt);
+                const Operand<KIND> b = operand(BN + col);
+                if constexpr (is_f8(KIND)) {
+                    const float f = sw * *reinterpret_cast<const float *>(stage + (BN + BT) * 128 + (col + r) * 4);
+#pragma unroll
+                    for (int s = 0; s < SN; ++s) {
+                        const f32x4 p = product<KIND>(a[s], b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[s][j][i] = __builtin_fmaf(p[i], f, acc[s][j][i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < SN; ++s) acc[s][j] = product<KIND>(a[s], b, acc[s][j]);
+                }
+            }
+        }
+        meet<0>();                                           // no load may land after the workgroup has ended
+        const float nan = __builtin_nanf("");
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int c = 16 * (j * WT + wt) + r;
+            if (c >= work.live) continue;
+            const int64_t i = static_cast<int64_t>(work.first) + c, row = target_row(A, i);
+            if (row < 0) continue;
+            const bool bad = source_row(A, i) < 0;
+#pragma unroll
+            for (int s = 0; s < SN; ++s) {
+                const int n = n0 + 16 * (SN * wn + s) + 4 * q;
+                if (n >= A.rows) continue;
+                f32x4 v = acc[s][j];
+                if (A.bias) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(work.group) * A.rows + n + e];
+                }
+                store4(A, row, n, bad ? f32x4{nan, nan, nan, nan} : v);
+            }
+        }
+    };
+    // the wave columns' most live 16-token columns, the same for all waves (they meet at the barriers)
+    const int nt = (live_cols + WT - 1) / WT;
+    if constexpr (ST >= 8) {
+        if (nt > 6) return run(std::integral_constant<int, 8>{});
+        if (nt > 5) return run(std::integral_constant<int, 6>{});
+        if (nt > 4) return run(std::integral_constant<int, 5>{});
+    }
+    if constexpr (ST >= 4) {
+        if (nt > 3) return run(std::integral_constant<int, 4>{});
+        if (nt > 2) return run(std::integral_constant<int, 3>{});
+    }
+    if (nt > 1) return run(std::integral_constant<int, 2>{});
+    run(std::integral_constant<int, 1>{});
+}
+
 // Most token tiles of `tile_rows` that n_rows rows in n_groups groups can have.
 int64_t most_token_tiles(const ProductArgs & a, int tile_rows) {
     const int64_t whole = (a.n_rows + tile_rows - 1) / tile_rows;
@@ -321,12 +547,25 @@ void launch_few_rows(const ProductArgs & a, hipStream_t stream) {
     check_hip(hipGetLastError(), "product launch");
 }
 
+template <int KIND, int SN, int ST, int WN, int WT, int STAGES>
+void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
+    constexpr int BN = 16 * SN * WN, BT = 16 * ST * WT;
+    const int64_t row_tiles = (a.rows + BN - 1) / BN, items = row_tiles * most_token_tiles(a, BT);
+    require(items < (int64_t{1} << 32) / (WN * WT * 64) - 8, "too many outputs for one launch");
+    hipLaunchKernelGGL((many_rows_kernel<KIND, SN, ST, WN, WT, STAGES>), dim3(static_cast<unsigned>((items + 7) / 8 * 8)),
+                       dim3(WN * WT * 64), 0, stream, a, static_cast<int>(row_tiles));
+    check_hip(hipGetLastError(), "product launch");
+}
+
 template <int KIND>
 void launch_product(const ProductArgs & a, hipStream_t stream) {
-    if (a.n_rows == 0 || a.rows == 0) return;
-    const int64_t mean = a.n_rows / std::min<int64_t>(a.n_groups, a.n_rows);
-    if (mean <= 16) launch_few_rows<KIND, 1, 1, 4>(a, stream);
-    else launch_few_rows<KIND, 4, 2, 4>(a, stream);
+    const int64_t groups = std::min<int64_t>(a.n_groups, a.n_rows), mean = a.n_rows / groups;
+    if (mean <= 16) return launch_few_rows<KIND == kF8 ? kF8Wide : KIND, 1, 1, 4>(a, stream);
+    auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
+    if (mean <= 32) launch_few_rows<KIND == kF8 ? kF8Wide : KIND, 4, 2, 4>(a, stream);
+    else if (tiles(256, 256) >= 192) launch_many_rows<KIND, 4, 8, 4, 2, 2>(a, stream);
+    else if (tiles(128, 128) >= 192) launch_many_rows<KIND, 4, 4, 2, 2, 2>(a, stream);
+    else launch_many_rows<KIND, 2, 2, 2, 2, 3>(a, stream);
 }
 
 void product(const vbm_weights & w, const void * b, const float * b_scales, ProductArgs a, int dst_type, void * dst, hipStream_t stream) {
@@ -358,7 +597,8 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     a.rows = static_cast<int>(w.rows);
     a.k_bytes = static_cast<int>(k_bytes);
     a.kb = static_cast<int>((k_bytes + 127) / 128);
-    if (f8) launch_product<kF8Wide>(a, stream);
+    if (f8 && dst_type != VBM_TYPE_F32) launch_product<kF8>(a, stream);
+    else if (f8) launch_product<kF8Wide>(a, stream);
     else if (w.type == VBM_TYPE_F16) launch_product<kF16>(a, stream);
     else launch_product<kBF16>(a, stream);
 }
