@@ -49,7 +49,8 @@ struct ProductArgs {
     const int32_t * dst_rows;      // grouped row -> dst row, or null
     int64_t n_dst;
     void * dst;
-    int dst_type, dst_vec;         // dst_vec: four neighbouring outputs can be stored at once
+    int dst_type;
+    int dst_vec, dst_vec16;        // four neighbouring outputs, or 16 bytes of them, can be stored at once
     int n_groups, rows, k_bytes, kb;
 };
 
@@ -121,13 +122,8 @@ struct Piece {
     u32x4p lo, hi;
 };
 
-__device__ __forceinline__ uint16_t to_bf16(float v) {   // nearest even; NaN stays NaN
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    if (v != v) return 0x7FC0;
-    return static_cast<uint16_t>((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-}
 __device__ __forceinline__ uint16_t to_16(int type, float v) {
-    return type == VBM_TYPE_BF16 ? to_bf16(v) : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+    return type == VBM_TYPE_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)) : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
 }
 
 // Outputs n .. n + 3 of one dst row.
@@ -314,9 +310,6 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(ProductArgs A, int row
 }
 
 // ----------------------------------------------------------------------------------- many tokens
-// Tokens of a step and row's zero pieces past its end.
-__device__ const u32x4p zero_piece[1] = {};
-
 // Loads from memory to LDS (lane l's bytes land at m0 + l * size), in inline assembly so that the compiler does not wait for
 // all of them before every LDS read; the kernel waits itself before each barrier. The compiler knows of no other use of
 // M0 here, and the wait state between a scalar write of M0 and the load that reads it is written out.
@@ -325,14 +318,69 @@ __device__ const u32x4p zero_piece[1] = {};
 __device__ __forceinline__ void load_to_lds_16(const void * src, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
 }
-__device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
+__device__ __forceinline__ void load_to_lds_16(const void * base, uint32_t offset, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(base), "v"(offset), "s"(m0) : "memory", "m0");
+}
+// (with `lanes` none of a wave's, the load counts as one and brings nothing; all lanes are active where it is called)
+__device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0, int lanes) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1" ::"v"(src), "s"(m0), "s"(lanes) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 // Waits until all but the wave's newest N loads have landed and its LDS reads are done, then for the workgroup's other waves.
 template <int N>
 __device__ __forceinline__ void meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Sixteen tokens' outputs from n on, fp32 in LDS (`row_bytes` a token), to their dst rows: PIECES of N values a token.
+template <int PIECES, int N>
+__device__ __forceinline__ void store_column(const ProductArgs & A, const uint8_t * from, int row_bytes, const int64_t * rows, int n) {
+    constexpr int AT_ONCE = 64 / PIECES;                     // tokens
+    const int lane = threadIdx.x & 63, at = n + lane % PIECES * N;
+#pragma unroll
+    for (int t = lane / PIECES; t < 16; t += AT_ONCE) {
+        const f32x4 * v4 = reinterpret_cast<const f32x4 *>(from + t * row_bytes + lane % PIECES * N * 4);
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v4[i / 4][i % 4];
+        int64_t row = rows[t];
+        if (row == -1 || at >= A.rows) continue;
+        if (row < 0) {
+            row = -2 - row;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __builtin_nanf("");
+        }
+        if constexpr (N == 4) {
+            float * p = static_cast<float *>(A.dst) + row * A.rows + at;
+            if (A.dst_vec16) {
+                *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (at + i < A.rows) p[i] = v[i];
+        } else {
+            uint16_t * p = static_cast<uint16_t *>(A.dst) + row * A.rows + at;
+            uint16_t h[N];
+            if (A.dst_type == VBM_TYPE_BF16) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[i] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(v[i]));
+            }
+            if (A.dst_vec16) {
+                u32x4p w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
+                *reinterpret_cast<u32x4p *>(p) = w;
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (at + i < A.rows) p[i] = h[i];
+        }
+    }
 }
 
 struct Work {
@@ -390,15 +438,14 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 
 // A workgroup of WN x WT waves takes BN = 16 SN WN weight rows x up to BT = 16 ST WT tokens of one group; a wave 16 SN rows x every WT-th
 // 16-token column. A step's 128 bytes of every row are staged in LDS, STAGES - 1 steps ahead, with one wait and one barrier a
-// step. Piece p (16 bytes) of row r lies at place p ^ (r & 7) of the row's 128 bytes, so that sixteen rows' reads of one piece
-// spread over the banks.
+// step. Piece p (16 bytes) of row r lies at place p ^ (r / 2 % 8) of the row's 128 bytes, so that sixteen rows' reads of one piece
+// cover all 64 banks once (with p ^ (r % 8) rows r and r + 8 met in the same ones, and every read took twice as long).
 template <int KIND, int SN, int ST, int WN, int WT, int STAGES>
 __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
     constexpr int DW = BN / 8 / W, DT = BT / 8 / W;          // a wave's loads a step: 8 rows each
     static_assert(DW * 8 * W == BN && DT * 8 * W == BT && BT % 64 == 0, "the waves share the loads evenly");
     constexpr int STAGE = (BN + BT) * 128 + (is_f8(KIND) ? BT * 4 : 0);
-    constexpr int PER_STEP = DW + DT + (is_f8(KIND) ? 1 : 0);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
     Work work;
     if (!find_work(A, ST * WT, row_tiles, work)) return;
@@ -407,12 +454,16 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     const int n0 = work.row_tile * BN;
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
 
-    const uint8_t * wsrc[DW], * tsrc[DT];
-    const int piece = (lane & 7) ^ (lane >> 3);              // the one this lane brings of row lane / 8 of eight
+    const uint8_t * wbase = A.w + (static_cast<int64_t>(work.group) * A.rows + n0) * A.k_bytes, * tsrc[DT];
+    uint32_t wsrc[DW];                                       // (rows of a tile are at most 2^32 bytes apart)
+    // the piece that this lane brings of row lane / 8 of eight: place lane % 8, of rows 0 .. 7 or 8 .. 15 of sixteen (loads k = wave + W i
+    // with even or odd k; W is even, so all of a wave's are alike)
+    static_assert(W % 2 == 0, "a wave's loads are all of even or all of odd eights");
+    const int piece = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
 #pragma unroll
     for (int i = 0; i < DW; ++i) {
         const int n = n0 + 8 * (wave + W * i) + (lane >> 3);
-        wsrc[i] = A.w + (static_cast<int64_t>(work.group) * A.rows + (n < A.rows ? n : A.rows - 1)) * A.k_bytes + piece * 16;
+        wsrc[i] = static_cast<uint32_t>((n < A.rows ? n : A.rows - 1) - n0) * static_cast<uint32_t>(A.k_bytes) + piece * 16;
     }
     auto token_row = [&](int i) __attribute__((always_inline)) {   // spare tokens repeat the first one, unknown ones read row 0
         const int64_t src = source_row(A, work.first + (i < work.live ? i : 0));
@@ -420,7 +471,8 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     };
 #pragma unroll
     for (int i = 0; i < DT; ++i) tsrc[i] = A.b + token_row(8 * (wave + W * i) + (lane >> 3)) * A.k_bytes + piece * 16;
-    const int scale_slot = wave % (BT / 64);
+    const int scale_slot = wave % (BT / 64);                 // the first BT / 64 waves bring the tokens' scales
+    const int scale_lanes = (wave - BT / 64) >> 31;
     const float * ssrc = nullptr, * wscale = nullptr;
     if constexpr (is_f8(KIND)) {
         ssrc = A.bs + token_row(64 * scale_slot + lane) * A.kb;
@@ -429,23 +481,10 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     }
 
     const int live_cols = (work.live + 15) >> 4;
-    auto issue = [&](int kb) __attribute__((always_inline)) {
-        const uint32_t at = lds0 + (kb % STAGES) * STAGE;
-        const int k = kb < A.kb ? kb : A.kb - 1;             // (past the end: the last step again, into a stage that nobody reads)
-        const bool past = k * 128 + piece * 16 >= A.k_bytes;
-        auto from = [&](const uint8_t * p) __attribute__((always_inline)) {
-            return past ? reinterpret_cast<const uint8_t *>(zero_piece) : p + static_cast<int64_t>(k) * 128;
-        };
-#pragma unroll
-        for (int i = 0; i < DW; ++i) load_to_lds_16(from(wsrc[i]), at + (wave + W * i) * 1024);
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-            if (STAGES > 2 || 8 * (wave + W * i) < 16 * live_cols) load_to_lds_16(from(tsrc[i]), at + BN * 128 + (wave + W * i) * 1024);
-        if constexpr (is_f8(KIND)) load_to_lds_4(ssrc + k, at + (BN + BT) * 128 + scale_slot * 256);
-    };
-
     auto run = [&](auto live_c) __attribute__((always_inline)) {
         constexpr int NT = decltype(live_c)::value;
+        constexpr int LOADS = DW + (NT * WT * 2 + W - 1) / W;                 // only the live columns' tokens
+        constexpr int PARTS = LOADS + (is_f8(KIND) ? 1 : 0);
         f32x4 acc[SN][NT];
 #pragma unroll
         for (int s = 0; s < SN; ++s)
@@ -454,67 +493,163 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         float scales = 0.0f;                                 // lane l: the weights' scale of step l (mod 64)
         auto fetch_scales = [&](int kb) __attribute__((always_inline)) {
             if constexpr (is_f8(KIND)) scales = kb + lane < A.kb ? wscale[kb + lane] : 0.0f;
+            asm volatile("" : "+v"(scales));                 // (the wait for it here, not in every step, where it would wait for the stages too)
         };
-        fetch_scales(0);
+        // Loads [begin, end) of a step's PARTS (weights, tokens, the tokens' scales) into stage `to`. A stage's loads go out a few (EACH) a
+        // column, from the last column of the step that frees it on: together they would hold up the reads and products behind them, and
+        // later ones would not have landed in time. Past the last step it is loaded again, for nobody, so that the waits' counts
+        // hold; a piece past a row's end reads the step's first one (zeros take its place before it is used).
+        constexpr int EACH = (PARTS + NT / 2) / (NT / 2 + 1);
+        auto load_parts = [&](int to, int begin, int end) __attribute__((always_inline)) {
+            const int kb = to < A.kb ? to : A.kb - 1;
+            const int64_t off = static_cast<int64_t>(kb) * 128;
+            const int back = kb * 128 + piece * 16 < A.k_bytes ? 0 : -16 * piece;
+            const uint32_t at = lds0 + (to % STAGES) * STAGE;
 #pragma unroll
-        for (int kb = 0; kb < STAGES - 1; ++kb) issue(kb);
-        const int lo = r * 128 + ((2 * q) ^ (r & 7)) * 16, hi = r * 128 + ((2 * q + 1) ^ (r & 7)) * 16;
-        for (int kb = 0; kb < A.kb; ++kb) {
-            meet<(STAGES - 2) * PER_STEP>();
-            if (STAGES > 2 || kb + 1 < A.kb) issue(kb + STAGES - 1);
-            const uint8_t * stage = lds + (kb % STAGES) * STAGE;
-            auto operand = [&](int row) __attribute__((always_inline)) {
-                Operand<KIND> o;
-                o.take(Piece{*reinterpret_cast<const u32x4p *>(stage + row * 128 + lo), *reinterpret_cast<const u32x4p *>(stage + row * 128 + hi)});
-                return o;
-            };
-            Operand<KIND> a[SN];
+            for (int i = begin; i < end; ++i) {
+                if (i < DW) load_to_lds_16(wbase + off, wsrc[i < DW ? i : 0] + back, at + (wave + W * i) * 1024);
+                else if (i < LOADS) load_to_lds_16(tsrc[i - DW < DT ? i - DW : 0] + off + back, at + BN * 128 + (wave + W * (i - DW)) * 1024);
+                else load_to_lds_4(ssrc + kb, at + (BN + BT) * 128 + scale_slot * 256, scale_lanes);
+            }
+        };
 #pragma unroll
-            for (int s = 0; s < SN; ++s) a[s] = operand(16 * (SN * wn + s));
+        for (int kb = 0; kb < STAGES; ++kb) load_parts(kb, 0, kb == STAGES - 1 ? EACH : PARTS);
+        // this lane's places in a stage: pieces 2q and 2q + 1 of row r of sixteen, and the token columns' scales
+        const uint32_t lo = r * 128 + ((2 * q) ^ (r >> 1)) * 16, hi = r * 128 + ((2 * q + 1) ^ (r >> 1)) * 16;
+        constexpr int COL = 16 * WT;                         // rows from one of a wave's token columns to the next
+        uint32_t a_lo, a_hi, b_lo, b_hi, b_scale;
+        auto enter = [&](int kb) __attribute__((always_inline)) {
+            const uint32_t stage = (kb % STAGES) * STAGE;
+            a_lo = stage + 2048 * SN * wn + lo, a_hi = stage + 2048 * SN * wn + hi;
+            b_lo = stage + BN * 128 + 2048 * wt + lo, b_hi = stage + BN * 128 + 2048 * wt + hi;
+            b_scale = stage + (BN + BT) * 128 + 64 * wt + 4 * r;
+            asm volatile("" : "+v"(a_lo), "+v"(a_hi), "+v"(b_lo), "+v"(b_hi), "+v"(b_scale));   // (offsets then fit the reads' own)
+        };
+        auto operand = [&](uint32_t at_lo, uint32_t at_hi, int rows) __attribute__((always_inline)) {
+            Operand<KIND> o;
+            o.take(Piece{*reinterpret_cast<const u32x4p *>(lds + at_lo + rows * 128), *reinterpret_cast<const u32x4p *>(lds + at_hi + rows * 128)});
+            return o;
+        };
+        auto token_scale = [&](int j) __attribute__((always_inline)) {
+            return *reinterpret_cast<const float *>(lds + b_scale + j * COL * 4);
+        };
+        // Software pipeline over the columns: the products p[s] of a column are summed under the matrix instructions of the next one, whose
+        // operand is read a column ahead. Before a step's last column the waves meet: the next step's stage has landed, and this
+        // step's has been read (its last operands are in registers) and takes the bytes of a later one; the next step's
+        // first operands are read under the last column, the weights' into the registers that it has just used.
+        Operand<KIND> a[SN], b[2];
+        float sb[2] = {0.0f, 0.0f}, factor = 0.0f;
+        f32x4 p[SN];
+#pragma unroll
+        for (int s = 0; s < SN; ++s) p[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        auto first_operands = [&](int kb) __attribute__((always_inline)) {
+            enter(kb);
+            b[0] = operand(b_lo, b_hi, 0);
+            if constexpr (is_f8(KIND)) sb[0] = token_scale(0);
+#pragma unroll
+            for (int s = 0; s < SN; ++s) a[s] = operand(a_lo, a_hi, 16 * s);
+        };
+        meet<(STAGES - 2) * PARTS + EACH>();
+        first_operands(0);
+        auto step = [&](int kb, auto more_c) __attribute__((always_inline)) {
+            constexpr bool MORE = decltype(more_c)::value;   // another step follows
             float sw = 0.0f;
             if constexpr (is_f8(KIND)) {
-                if (kb && !(kb & 63)) fetch_scales(kb);
                 sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scales), kb & 63));
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int col = 16 * (j * WT + wt);
-                const Operand<KIND> b = operand(BN + col);
-                if constexpr (is_f8(KIND)) {
-                    const float f = sw * *reinterpret_cast<const float *>(stage + (BN + BT) * 128 + (col + r) * 4);
+                const bool last = j + 1 == NT, read = !last || MORE;
+                if (last && MORE) {
+                    meet<(STAGES - 2) * PARTS>();
+                    enter(kb + 1);
+                }
+                const Operand<KIND> now = b[j & 1];
+                const float scale_now = sb[j & 1];
+                const int next = last ? 0 : (j + 1) & 1;
+                if (read) b[next] = operand(b_lo, b_hi, last ? 0 : (j + 1) * COL);
+                if (is_f8(KIND) && read) sb[next] = token_scale(last ? 0 : j + 1);
+                const int before = j ? j - 1 : NT - 1;
+#pragma unroll
+                for (int s = 0; s < SN; ++s) {
+                    if constexpr (is_f8(KIND)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[s][before][i] = __builtin_fmaf(p[s][i], factor, acc[s][before][i]);
+                        p[s] = product<KIND>(a[s], now, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    } else {
+                        acc[s][j] = product<KIND>(a[s], now, acc[s][j]);
+                    }
+                    if (last && MORE) a[s] = operand(a_lo, a_hi, 16 * s);
+                }
+                if constexpr (is_f8(KIND)) factor = sw * scale_now;
+                // (left to itself the compiler sums a product right behind its matrix instruction and waits for it)
+                if constexpr (KIND == kF8) {
+                    if (read) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);          // the next column's reads
 #pragma unroll
                     for (int s = 0; s < SN; ++s) {
-                        const f32x4 p = product<KIND>(a[s], b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[s][j][i] = __builtin_fmaf(p[i], f, acc[s][j][i]);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);                  // a product's sums,
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                  // the next product
+                        if (last && MORE) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                     }
-                } else {
-#pragma unroll
-                    for (int s = 0; s < SN; ++s) acc[s][j] = product<KIND>(a[s], b, acc[s][j]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                if (last && MORE) load_parts(kb + STAGES, 0, EACH);
+                if (!last && MORE) load_parts(kb + STAGES - 1, std::min((j + 1) * EACH, PARTS), std::min((j + 2) * EACH, PARTS));
             }
+        };
+        const int whole = A.k_bytes >> 7;
+        for (int kb = 0; kb < whole;) {
+            fetch_scales(kb);
+            const int end = kb + 64 < whole ? kb + 64 : whole;
+            for (; kb < end; ++kb) step(kb, std::true_type{});   // (no branch inside a step: the compiler would move sums behind it)
+        }
+        if (whole < A.kb) {                                  // a row's last bytes, less than a step
+            if (!(whole & 63)) fetch_scales(whole);
+            if (whole * 128 + piece * 16 >= A.k_bytes) {
+                uint8_t * mine = lds + (whole % STAGES) * STAGE + wave * 1024 + lane * 16;
+#pragma unroll
+                for (int i = 0; i < DW; ++i) *reinterpret_cast<u32x4p *>(mine + W * i * 1024) = u32x4p{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < LOADS - DW; ++i) *reinterpret_cast<u32x4p *>(mine + BN * 128 + W * i * 1024) = u32x4p{0, 0, 0, 0};
+            }
+            meet<0>();
+            first_operands(whole);
+            step(whole, std::false_type{});
+        }
+        if constexpr (is_f8(KIND)) {
+#pragma unroll
+            for (int s = 0; s < SN; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[s][NT - 1][i] = __builtin_fmaf(p[s][i], factor, acc[s][NT - 1][i]);
         }
         meet<0>();                                           // no load may land after the workgroup has ended
-        const float nan = __builtin_nanf("");
+        // A wave's 16-token column at a time goes through LDS, so that neighbouring lanes store neighbouring bytes of a dst row:
+        // straight from the registers (16 rows x 32 bytes a store) the stores of a 4096 x 4096 output took 6 us longer.
+        constexpr int ROW = 16 * SN * 4 + 16;                // bytes of a token's outputs there
+        static_assert(W * 16 * ROW + BT * 8 <= STAGES * STAGE, "the stages' memory holds them");
+        int64_t * rows = reinterpret_cast<int64_t *>(lds + W * 16 * ROW);   // dst row, -1: none, -2 - row: all NaN
+        for (int c = threadIdx.x; c < BT; c += W * 64) {
+            const int64_t i = static_cast<int64_t>(work.first) + c, row = c < work.live ? target_row(A, i) : -1;
+            rows[c] = row >= 0 && source_row(A, i) < 0 ? -2 - row : row;
+        }
+        __syncthreads();
+        const int nw = n0 + 16 * SN * wn;                    // the wave's first output
+        f32x4 bias[SN];
+#pragma unroll
+        for (int s = 0; s < SN; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = nw + 16 * s + 4 * q + e;
+                bias[s][e] = A.bias && n < A.rows ? A.bias[static_cast<int64_t>(work.group) * A.rows + n] : 0.0f;
+            }
+        uint8_t * mine = lds + wave * 16 * ROW;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int c = 16 * (j * WT + wt) + r;
-            if (c >= work.live) continue;
-            const int64_t i = static_cast<int64_t>(work.first) + c, row = target_row(A, i);
-            if (row < 0) continue;
-            const bool bad = source_row(A, i) < 0;
 #pragma unroll
-            for (int s = 0; s < SN; ++s) {
-                const int n = n0 + 16 * (SN * wn + s) + 4 * q;
-                if (n >= A.rows) continue;
-                f32x4 v = acc[s][j];
-                if (A.bias) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(work.group) * A.rows + n + e];
-                }
-                store4(A, row, n, bad ? f32x4{nan, nan, nan, nan} : v);
-            }
+            for (int s = 0; s < SN; ++s) *reinterpret_cast<f32x4 *>(mine + r * ROW + 64 * s + 16 * q) = acc[s][j] + bias[s];
+            const int64_t * to = rows + 16 * (j * WT + wt);
+            if (A.dst_type == VBM_TYPE_F32) store_column<4 * SN, 4>(A, mine, ROW, to, nw);
+            else store_column<2 * SN, 8>(A, mine, ROW, to, nw);
         }
     };
     // the wave columns' most live 16-token columns, the same for all waves (they meet at the barriers)
@@ -563,7 +698,7 @@ void launch_product(const ProductArgs & a, hipStream_t stream) {
     if (mean <= 16) return launch_few_rows<KIND == kF8 ? kF8Wide : KIND, 1, 1, 4>(a, stream);
     auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
     if (mean <= 32) launch_few_rows<KIND == kF8 ? kF8Wide : KIND, 4, 2, 4>(a, stream);
-    else if (tiles(256, 256) >= 192) launch_many_rows<KIND, 4, 8, 4, 2, 2>(a, stream);
+    else if (KIND != kF8Wide && tiles(256, 256) >= 192) launch_many_rows<KIND == kF8Wide ? kF8 : KIND, 4, 8, 4, 2, 2>(a, stream);
     else if (tiles(128, 128) >= 192) launch_many_rows<KIND, 4, 4, 2, 2, 2>(a, stream);
     else launch_many_rows<KIND, 2, 2, 2, 2, 3>(a, stream);
 }
@@ -573,7 +708,7 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     require(f8 || w.type == VBM_TYPE_F16 || w.type == VBM_TYPE_BF16, "weights must be F8_E4M3, F16 or BF16");
     require(dst_type == VBM_TYPE_F32 || dst_type == VBM_TYPE_F16 || dst_type == VBM_TYPE_BF16, "dst must be F32, F16 or BF16");
     require(w.n_groups > 0 && w.n_groups <= 1024, "n_groups must be in 1..1024");
-    require(w.rows > 0 && w.rows < (int64_t{1} << 30) && w.k > 0 && w.k < (int64_t{1} << 29), "rows and k out of range");
+    require(w.rows > 0 && w.rows < (int64_t{1} << 30) && w.k > 0 && w.k < (int64_t{1} << 23), "rows and k out of range");
     const int64_t k_bytes = w.k * (f8 ? 1 : 2);
     require(k_bytes % 16 == 0, f8 ? "k must be a multiple of 16" : "k must be a multiple of 8");
     require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 31) && a.n_b >= 0 && a.n_dst >= 0, "row counts out of range");
@@ -593,6 +728,7 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     a.dst = dst;
     a.dst_type = dst_type;
     a.dst_vec = at(dst, 4 * dsize) && w.rows % 4 == 0;
+    a.dst_vec16 = at(dst, 16) && static_cast<size_t>(w.rows) * dsize % 16 == 0;
     a.n_groups = static_cast<int>(w.n_groups);
     a.rows = static_cast<int>(w.rows);
     a.k_bytes = static_cast<int>(k_bytes);
