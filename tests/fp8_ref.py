@@ -112,17 +112,18 @@ LEAST_STEP = {vb.TYPE_F32: 0.0, vb.TYPE_F16: 2.0 ** -25, vb.TYPE_BF16: 0.0}   # 
 
 
 class Matrix:
-    """Device weights of a vbm_weights, and their float64 values."""
+    """Device weights of a vbm_weights, and the float64 values of their first `distinct` groups, which repeat."""
 
-    def __init__(self, type_id, rng, groups, rows, k, bias=False):
-        self.type_id, self.groups, self.rows, self.k = type_id, groups, rows, k
+    def __init__(self, type_id, rng, groups, rows, k, bias=False, distinct=None):
+        self.type_id, self.groups, self.rows, self.k, self.distinct = type_id, groups, rows, k, distinct or groups
+        repeated = lambda a: vb.DeviceBuffer.from_array(a[np.arange(groups) % self.distinct])  # noqa: E731
         if type_id == F8:
-            codes, scales = fp8_matrix(rng, groups, rows, k)
+            codes, scales = fp8_matrix(rng, self.distinct, rows, k)
             self.values = matrix_of(codes, scales)
-            self.data, self.scales = vb.DeviceBuffer.from_array(codes), vb.DeviceBuffer.from_array(scales)
+            self.data, self.scales = repeated(codes), repeated(scales)
         else:
-            raw, self.values = store_as(type_id, rng.standard_normal((groups, rows, k)) / np.sqrt(k))
-            self.data, self.scales = vb.DeviceBuffer.from_array(raw), None
+            raw, self.values = store_as(type_id, rng.standard_normal((self.distinct, rows, k)) / np.sqrt(k))
+            self.data, self.scales = repeated(raw), None
         self.bias_values = rng.standard_normal((groups, rows)).astype(np.float32) * np.float32(0.1) if bias else None
         self.bias = vb.DeviceBuffer.from_array(self.bias_values) if bias else None
         self.desc = vb.Weights(type_id, self.data.ptr, vb.ptr(self.scales), vb.ptr(self.bias), groups, rows, k)
@@ -193,7 +194,8 @@ def grouped_want(m, tokens, n_b, offsets, n_rows, n_dst, b_rows=None, b_div=1, d
         src, d = src[keep], d[keep]
         known = (src >= 0) & (src < n_b)
         x = tokens.values[np.where(known, src, 0)]
-        v, s = x @ m.values[g].T, np.abs(x) @ np.abs(m.values[g]).T
+        w = m.values[g % m.distinct]
+        v, s = x @ w.T, np.abs(x) @ np.abs(w).T
         if m.bias_values is not None:
             v, s = v + m.bias_values[g], s + np.abs(m.bias_values[g])
         y[d], size[d], written[d] = np.where(known[:, None], v, np.nan), s, True

@@ -195,6 +195,24 @@ def test_grouped_product_over_many_groups(gpu, type_id, groups):
     R.check(m, F32, got, *R.grouped_want(m, x, used, offsets, used, used), f"{groups} groups")
 
 
+@pytest.mark.parametrize("type_id,dst_type", [(F8, F32), (F8, BF16), (F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("groups,rows,k,most", [(140, 481, 336, 16), (1024, 64, 1808, 3), (70, 1037, 3296, 19), (300, 250, 6800, 9), (500, 161, 1024, 33)])
+def test_grouped_product_few_rows_of_many(gpu, type_id, dst_type, groups, rows, k, most):
+    """Some rows for each of many experts, at depths whose tokens do and do not fit on the chip."""
+    k = k if type_id == F8 else k // 2
+    rng = np.random.default_rng(groups + k)
+    counts = rng.integers(0, most + 1, groups)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    n_rows = int(offsets[-1]) + 2
+    place = rng.permutation(n_rows).astype(np.int32)
+    gather = k % 32 == 0
+    n_b = -(-n_rows // 2) if gather else n_rows
+    m, x = R.Matrix(type_id, rng, groups, rows, k, bias=True, distinct=4), R.Tokens(type_id, rng, n_b, k)
+    kw = dict(b_rows=place, b_div=2) if gather else dict(dst_rows=place)
+    got = R.grouped(m, x, n_b, offsets, n_rows, dst_type, n_rows, **kw)
+    R.check(m, dst_type, got, *R.grouped_want(m, x, n_b, offsets, n_rows, n_rows, **kw), f"few rows of {groups}")
+
+
 @pytest.mark.parametrize("type_id,dst_type", [(F8, F32), (F8, F16), (F8, BF16), (F16, F32), (BF16, BF16)])
 @pytest.mark.parametrize("gather", [True, False])
 @pytest.mark.parametrize("rows,k,groups,most", [(2100, 272, 24, 290), (1090, 400, 24, 290), (520, 656, 6, 290), (257, 1168, 3, 700)])

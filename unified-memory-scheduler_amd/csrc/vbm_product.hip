@@ -187,129 +187,6 @@ __device__ __forceinline__ f32x4 product(const Operand<KIND> & a, const Operand<
     return c;
 }
 
-// ------------------------------------------------------------------------------- few tokens a group
-// A workgroup takes 16 * RS weight rows x up to 16 * NT tokens of one group; its W waves share the depth and add their sums up
-// through LDS, in wave order. Weights and tokens go from memory to registers: with few tokens a group the weights'
-// bytes are the work, and nobody else in the workgroup needs them.
-template <int KIND, int NT, int RS, int W>
-__global__ __launch_bounds__(W * 64) void few_rows_kernel(ProductArgs A, int row_tiles) {
-    constexpr int U = NT * RS <= 2 ? 4 : 2;                  // steps whose loads go out together
-    __shared__ f32x4 parts[W][RS * NT][64];
-    TokenTile t;
-    const int token_tile = static_cast<int>(blockIdx.x) / row_tiles, n0 = (static_cast<int>(blockIdx.x) - token_tile * row_tiles) * (16 * RS);
-    if (!find_token_tile(A, token_tile, 16 * NT, t)) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const int q = lane >> 4, r = lane & 15;
-
-    // lane (q, r) brings 16-byte pieces q and q + 4 of a step: the four lanes of a row read 64 bytes side by side
-    const uint8_t * wp[RS], * bp[NT];
-    const float * bsp[NT], * wsp = nullptr;
-    bool bad[NT];
-#pragma unroll
-    for (int s = 0; s < RS; ++s) {
-        const int row = n0 + 16 * s + r < A.rows ? n0 + 16 * s + r : A.rows - 1;
-        wp[s] = A.w + (static_cast<int64_t>(t.group) * A.rows + row) * A.k_bytes + q * 16;
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int64_t i = t.first + 16 * j + r;
-        const int64_t src = source_row(A, i < t.last ? i : t.first);   // (spare columns repeat the tile's first token)
-        bad[j] = src < 0;
-        bp[j] = A.b + (bad[j] ? 0 : src) * A.k_bytes + q * 16;
-        if constexpr (is_f8(KIND)) bsp[j] = A.bs + (bad[j] ? 0 : src) * A.kb;
-    }
-    if constexpr (is_f8(KIND)) wsp = A.ws + (static_cast<int64_t>(t.group) * ((A.rows + 127) >> 7) + (n0 >> 7)) * A.kb;
-
-    f32x4 acc[RS][NT];
-#pragma unroll
-    for (int s = 0; s < RS; ++s)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    // UU steps from kb on; TAIL: the row's last step, whose pieces past the row are zeros
-    auto steps = [&](auto uu_c, auto tail_c, int kb) __attribute__((always_inline)) {
-        constexpr int UU = decltype(uu_c)::value;
-        constexpr bool TAIL = decltype(tail_c)::value;
-        const int left = A.k_bytes - kb * 128 - q * 16;       // bytes of the row from this lane's first piece on
-        auto piece = [&](const uint8_t * p, int u) __attribute__((always_inline)) {
-            const uint8_t * at = p + static_cast<int64_t>(kb + u) * 128;
-            Piece v{};
-            if (!TAIL || left > 0) v.lo = *reinterpret_cast<const u32x4p *>(at);
-            if (!TAIL || left > 64) v.hi = *reinterpret_cast<const u32x4p *>(at + 64);
-            return v;
-        };
-        Piece wv[UU][RS], bv[UU][NT];
-        float sc[UU][NT], sw[UU];
-#pragma unroll
-        for (int u = 0; u < UU; ++u) {
-#pragma unroll
-            for (int s = 0; s < RS; ++s) wv[u][s] = piece(wp[s], u);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) bv[u][j] = piece(bp[j], u);
-            if constexpr (is_f8(KIND)) {
-                sw[u] = wsp[kb + u];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) sc[u][j] = bsp[j][kb + u];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < UU; ++u) {
-            Operand<KIND> a[RS];
-#pragma unroll
-            for (int s = 0; s < RS; ++s) a[s].take(wv[u][s]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                Operand<KIND> b;
-                b.take(bv[u][j]);
-#pragma unroll
-                for (int s = 0; s < RS; ++s) {
-                    if constexpr (is_f8(KIND)) {
-                        const f32x4 p = product<KIND>(a[s], b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                        const float f = sw[u] * sc[u][j];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[s][j][i] = __builtin_fmaf(p[i], f, acc[s][j][i]);
-                    } else {
-                        acc[s][j] = product<KIND>(a[s], b, acc[s][j]);
-                    }
-                }
-            }
-        }
-    };
-    using One = std::integral_constant<int, 1>;
-    const int k_end = A.kb * (wave + 1) / W, whole = A.k_bytes >> 7;
-    int kb = A.kb * wave / W;
-    for (; kb + U <= (k_end < whole ? k_end : whole); kb += U) steps(std::integral_constant<int, U>{}, std::false_type{}, kb);
-    for (; kb < (k_end < whole ? k_end : whole); ++kb) steps(One{}, std::false_type{}, kb);
-    if (kb < k_end) steps(One{}, std::true_type{}, kb);
-
-#pragma unroll
-    for (int s = 0; s < RS; ++s)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) parts[wave][s * NT + j][lane] = acc[s][j];
-    __syncthreads();
-#pragma unroll
-    for (int f = 0; f < RS * NT; ++f) {
-        if (f % W != wave) continue;
-        const int s = f / NT, j = f % NT;
-        f32x4 v = parts[0][f][lane];
-#pragma unroll
-        for (int w = 1; w < W; ++w) v += parts[w][f][lane];
-        const int n = n0 + 16 * s + 4 * q;
-        const int64_t i = t.first + 16 * j + r;
-        if (i >= t.last || n >= A.rows) continue;
-        const int64_t row = target_row(A, i);
-        if (row < 0) continue;
-        if (A.bias) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(t.group) * A.rows + n + e];
-        }
-        const float nan = __builtin_nanf("");
-        store4(A, row, n, bad[j] ? f32x4{nan, nan, nan, nan} : v);
-    }
-}
-
-// ----------------------------------------------------------------------------------- many tokens
 // Loads from memory to LDS (lane l's bytes land at m0 + l * size), in inline assembly so that the compiler does not wait for
 // all of them before every LDS read; the kernel waits itself before each barrier. The compiler knows of no other use of
 // M0 here, and the wait state between a scalar write of M0 and the load that reads it is written out.
@@ -332,6 +209,353 @@ __device__ __forceinline__ void meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// All but the wave's newest N loads have landed, and its LDS reads are done.
+template <int N>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+// The last steps of a ring, at most LEFT + 1 of them, with P loads each on their way.
+template <int LEFT, int P, class F>
+__device__ __forceinline__ void drain(int i, int n, const F & compute) {
+    if (n - i > LEFT) {
+        landed<LEFT * P>();
+        compute(i);
+        ++i;
+    }
+    if constexpr (LEFT > 0) drain<LEFT - 1, P>(i, n, compute);
+}
+
+// ------------------------------------------------------------------------------- few tokens a group
+// A workgroup takes 16 * RS weight rows x up to 8 * MAX8 tokens of one group; its W waves share the depth in runs and add their
+// sums up through LDS, in wave order. The weights' bytes are the work, and they are read once; what counts is that enough of them
+// are on their way. Each wave streams its own through a ring of D steps in LDS, without barriers: a load brings 128
+// bytes of each of eight rows, in neighbouring lanes (loaded straight into a matrix operand's registers, 16 rows in neighbouring lanes,
+// a kilobyte occupies the address unit for 64 cycles instead of 18, which alone limits a CU to 16 bytes a cycle).
+template <int KIND, int MAX8, int RS, int D>
+__global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_tiles) {
+    constexpr int W = 4, NT_MAX = (MAX8 + 1) / 2, RUN = 16;  // RUN: steps whose scales a wave holds
+    constexpr int STEP = (2 * RS + MAX8) * 1024, SCALES = is_f8(KIND) ? RUN * 64 * NT_MAX : 0, WAVE = D * STEP + SCALES;
+    static_assert(W * RS * NT_MAX * 1024 <= W * WAVE, "the ring's memory holds the waves' sums");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[W * WAVE];
+    TokenTile t;
+    const int token_tile = static_cast<int>(blockIdx.x) / row_tiles, n0 = (static_cast<int>(blockIdx.x) - token_tile * row_tiles) * (16 * RS);
+    if (!find_token_tile(A, token_tile, 8 * MAX8, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int q = lane >> 4, r = lane & 15, live = static_cast<int>(t.last - t.first);
+    uint8_t * mine = lds + wave * WAVE;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(mine));
+    auto token_row = [&](int i) __attribute__((always_inline)) {   // spare tokens repeat the first one, unknown ones read row 0
+        const int64_t src = source_row(A, t.first + (i < live ? i : 0));
+        return src < 0 ? 0 : src;
+    };
+
+    const uint8_t * wbase = A.w + (static_cast<int64_t>(t.group) * A.rows + n0) * A.k_bytes;
+    uint32_t wsrc[2 * RS];
+#pragma unroll
+    for (int i = 0; i < 2 * RS; ++i) {
+        const int n = n0 + 8 * i + (lane >> 3);
+        wsrc[i] = static_cast<uint32_t>((n < A.rows ? n : A.rows - 1) - n0) * static_cast<uint32_t>(A.k_bytes);
+    }
+    const float * wscale = is_f8(KIND) ? A.ws + (static_cast<int64_t>(t.group) * ((A.rows + 127) >> 7) + (n0 >> 7)) * A.kb : nullptr;
+    const int k_begin = A.kb * wave / W, k_end = A.kb * (wave + 1) / W;
+
+    auto run = [&](auto t8_c) __attribute__((always_inline)) {
+        constexpr int T8 = decltype(t8_c)::value, NT = (T8 + 1) / 2, P = 2 * RS + T8;   // P: loads a step
+        const uint8_t * tsrc[T8];
+#pragma unroll
+        for (int i = 0; i < T8; ++i) tsrc[i] = A.b + token_row(8 * i + (lane >> 3)) * A.k_bytes;
+        const float * ssrc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ssrc[j] = is_f8(KIND) ? A.bs + token_row(16 * j + (lane >> 2)) * A.kb : nullptr;
+        // piece lane % 8 of a row sits at its place xor (row / 2 % 8), as in the kernels below
+        const int piece_even = (lane & 7) ^ (lane >> 4), piece_odd = piece_even ^ 4;
+        f32x4 acc[RS][NT];
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+        for (int k0 = k_begin; k0 < k_end; k0 += RUN) {
+            const int n_steps = k_end - k0 < RUN ? k_end - k0 : RUN;
+            float scales = 0.0f;                             // lane l: the weights' scale of step k0 + l
+            if constexpr (is_f8(KIND)) {
+                scales = lane < n_steps ? wscale[k0 + lane] : 0.0f;
+                asm volatile("" : "+v"(scales));
+                // the tokens' scales, four steps of sixteen tokens a load: [four steps][token][4]
+                for (int c = 0; c < (n_steps + 3) / 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const int k = k0 + 4 * c + (lane & 3);
+                        load_to_lds_4(ssrc[j] + (k < A.kb ? k : A.kb - 1), lds0 + D * STEP + (c * NT_MAX + j) * 256, -1);
+                    }
+            }
+            auto issue = [&](int i) __attribute__((always_inline)) {
+                const int k = k0 + i;
+                const int64_t off = static_cast<int64_t>(k) * 128;
+                const uint32_t at = lds0 + (i % D) * STEP;
+                // (a piece past the row's end reads the step's first one: zeros take its place in the registers)
+                const int even = k * 128 + piece_even * 16 < A.k_bytes ? piece_even * 16 : 0, odd = k * 128 + piece_odd * 16 < A.k_bytes ? piece_odd * 16 : 0;
+#pragma unroll
+                for (int l = 0; l < 2 * RS; ++l) load_to_lds_16(wbase + off, wsrc[l] + (l & 1 ? odd : even), at + l * 1024);
+#pragma unroll
+                for (int l = 0; l < T8; ++l) load_to_lds_16(tsrc[l] + off + (l & 1 ? odd : even), at + (2 * RS + l) * 1024);
+            };
+            auto compute = [&](int i) __attribute__((always_inline)) {
+                const uint8_t * stage = mine + (i % D) * STEP;
+                const int left = A.k_bytes - (k0 + i) * 128 - 32 * q;   // bytes of the row from this lane's pieces on
+                auto operand = [&](int row) __attribute__((always_inline)) {
+                    // row r of sixteen; of eight tokens rows 8 .. 15 read rows 0 .. 7 (their columns are not used)
+                    const int rr = row >= 2 * RS * 8 && T8 == 1 ? r & 7 : r;
+                    const uint8_t * p = stage + row * 128 + rr * 128;
+                    Piece v{*reinterpret_cast<const u32x4p *>(p + ((2 * q) ^ (rr >> 1)) * 16), *reinterpret_cast<const u32x4p *>(p + ((2 * q + 1) ^ (rr >> 1)) * 16)};
+                    if (left < 32) {
+                        if (left <= 16) v.hi = u32x4p{0, 0, 0, 0};
+                        if (left <= 0) v.lo = u32x4p{0, 0, 0, 0};
+                    }
+                    Operand<KIND> o;
+                    o.take(v);
+                    return o;
+                };
+                Operand<KIND> a[RS];
+#pragma unroll
+                for (int s = 0; s < RS; ++s) a[s] = operand(16 * s);
+                float sw = 0.0f;
+                if constexpr (is_f8(KIND)) sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scales), i));
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const Operand<KIND> b = operand(16 * (RS + j));
+                    if constexpr (is_f8(KIND)) {
+                        const float f = sw * *reinterpret_cast<const float *>(mine + D * STEP + ((i >> 2) * NT_MAX + j) * 256 + r * 16 + (i & 3) * 4);
+#pragma unroll
+                        for (int s = 0; s < RS; ++s) {
+                            const f32x4 p = product<KIND>(a[s], b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[s][j][e] = __builtin_fmaf(p[e], f, acc[s][j][e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < RS; ++s) acc[s][j] = product<KIND>(a[s], b, acc[s][j]);
+                    }
+                }
+            };
+            for (int i = 0; i < D && i < n_steps; ++i) issue(i);
+            int i = 0;
+            for (; i + D < n_steps; ++i) {
+                landed<(D - 1) * P>();
+                compute(i);
+                landed<(D - 1) * P>();                       // (its reads are done: the wait covers them too)
+                issue(i + D);
+            }
+            drain<D - 1, P>(i, n_steps, compute);
+        }
+        __syncthreads();                                     // the rings are free: the waves' sums go there
+        f32x4 * parts = reinterpret_cast<f32x4 *>(lds);      // [wave][fragment][lane]
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) parts[(wave * RS * NT + s * NT + j) * 64 + lane] = acc[s][j];
+        __syncthreads();
+#pragma unroll
+        for (int f = 0; f < RS * NT; ++f) {
+            if (f % W != wave) continue;
+            const int s = f / NT, j = f % NT;
+            f32x4 v = parts[f * 64 + lane];
+#pragma unroll
+            for (int w = 1; w < W; ++w) v += parts[(w * RS * NT + f) * 64 + lane];
+            const int n = n0 + 16 * s + 4 * q;
+            const int64_t i = t.first + 16 * j + r;
+            if (i >= t.last || n >= A.rows) continue;
+            const int64_t row = target_row(A, i);
+            if (row < 0) continue;
+            if (A.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(t.group) * A.rows + n + e];
+            }
+            const float nan = __builtin_nanf("");
+            store4(A, row, n, source_row(A, i) < 0 ? f32x4{nan, nan, nan, nan} : v);
+        }
+    };
+    const int eights = (live + 7) >> 3;
+    if constexpr (MAX8 >= 4) {
+        if (eights > 2) return run(std::integral_constant<int, 4>{});
+    }
+    if constexpr (MAX8 >= 2) {
+        if (eights > 1) return run(std::integral_constant<int, 2>{});
+    }
+    run(std::integral_constant<int, 1>{});
+}
+
+// The same where there are rows enough to keep the card busy with one wave a row tile: the tokens, of all of the depth, are staged in LDS
+// once and shared by the workgroup's W waves; then each wave streams `tiles` row tiles of 16 rows, one after the other through
+// a ring of D steps, with no barrier and no sums to join.
+template <int KIND, int MAX8, int W, int D>
+struct StreamLayout {
+    static constexpr int NT = (MAX8 + 1) / 2, MAX_TILES = 4;
+    static constexpr int TOTAL = W * 20 * 1024;              // two workgroups of 4 waves, or one of 8, a CU
+    static constexpr int RING = W * D * 2048, ROWS = W * MAX_TILES * 16, BLOCKS = ROWS / 128 + 2;
+    static constexpr int BIAS = RING, BLOCK_SCALES = BIAS + ROWS * 4, TOKENS = BLOCK_SCALES + (is_f8(KIND) ? BLOCKS * 256 : 0);
+    static constexpr int STEP = MAX8 * 1024 + (is_f8(KIND) ? NT * 64 : 0);   // a step of the tokens and their scales
+    // steps that fit (scales come in fours; the weights' scales of 64 steps are kept)
+    static constexpr int FIT = (TOTAL - TOKENS - (is_f8(KIND) ? 4 * NT * 64 : 0)) / STEP;
+    static constexpr int MAX_KB = is_f8(KIND) && FIT > 64 ? 64 : FIT;
+};
+template <int KIND, int MAX8, int W, int D>
+__global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int row_units, int tiles) {
+    using L = StreamLayout<KIND, MAX8, W, D>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[L::TOTAL];
+    TokenTile t;
+    const int token_tile = static_cast<int>(blockIdx.x) / row_units, unit = static_cast<int>(blockIdx.x) - token_tile * row_units;
+    if (!find_token_tile(A, token_tile, 8 * MAX8, t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int q = lane >> 4, r = lane & 15, live = static_cast<int>(t.last - t.first), eights = (live + 7) >> 3;
+    const int n0 = unit * (W * 16) * tiles, row_tiles = (A.rows + 15) >> 4;
+    const int first_tile = (n0 >> 4) + wave;                 // this wave's: first_tile + W i
+    const int my_tiles = first_tile >= row_tiles ? 0 : ((row_tiles - first_tile + W - 1) / W < tiles ? (row_tiles - first_tile + W - 1) / W : tiles);
+    const uint8_t * weights = A.w + static_cast<int64_t>(t.group) * A.rows * A.k_bytes;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)), ring0 = lds0 + wave * (D * 2048);
+    const int piece_even = (lane & 7) ^ (lane >> 4), piece_odd = piece_even ^ 4;
+
+    // the weights' steps, in order over the wave's tiles: the next one to load is step kb_next of tile tile_next (the last one again past the end)
+    int tile_next = 0, kb_next = 0, slot_next = 0;
+    const uint8_t * base = nullptr;
+    uint32_t wsrc[2];
+    auto enter_tile = [&](int i) __attribute__((always_inline)) {
+        const int n = (first_tile + W * i) * 16;
+        base = weights + static_cast<int64_t>(n) * A.k_bytes;
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+            const int row = 8 * l + (lane >> 3);
+            wsrc[l] = static_cast<uint32_t>(n + row < A.rows ? row : A.rows - 1 - n) * static_cast<uint32_t>(A.k_bytes);
+        }
+    };
+    auto issue = [&]() __attribute__((always_inline)) {
+        const int64_t off = static_cast<int64_t>(kb_next) * 128;
+        // (a piece past the row's end reads the step's first one: zeros take its place in the registers)
+        const int even = kb_next * 128 + piece_even * 16 < A.k_bytes ? piece_even * 16 : 0, odd = kb_next * 128 + piece_odd * 16 < A.k_bytes ? piece_odd * 16 : 0;
+        load_to_lds_16(base + off, wsrc[0] + even, ring0 + slot_next * 2048);
+        load_to_lds_16(base + off, wsrc[1] + odd, ring0 + slot_next * 2048 + 1024);
+        slot_next = slot_next + 1 == D ? 0 : slot_next + 1;
+        if (kb_next + 1 < A.kb) {
+            ++kb_next;
+        } else if (tile_next + 1 < my_tiles) {
+            kb_next = 0;
+            enter_tile(++tile_next);
+        }
+    };
+    if (my_tiles) {
+        enter_tile(0);
+#pragma unroll
+        for (int i = 0; i < D; ++i) issue();
+    }
+
+    // the tokens: [eight tokens][step] x 1 KB, place as for the weights; scales [four steps][token][4]
+    auto token_row = [&](int i) __attribute__((always_inline)) {   // spare tokens repeat the first one, unknown ones read row 0
+        const int64_t src = source_row(A, t.first + (i < live ? i : 0));
+        return src < 0 ? 0 : src;
+    };
+    for (int e = 0; e < eights; ++e) {
+        const uint8_t * src = A.b + token_row(8 * e + (lane >> 3)) * A.k_bytes;
+        const int piece = e & 1 ? piece_odd : piece_even;
+        for (int kb = wave; kb < A.kb; kb += W) {
+            const uint32_t at = L::TOKENS + (e * A.kb + kb) * 1024;
+            if (kb * 128 + piece * 16 < A.k_bytes) load_to_lds_16(src + static_cast<int64_t>(kb) * 128 + piece * 16, lds0 + at);
+            else *reinterpret_cast<u32x4p *>(lds + at + lane * 16) = u32x4p{0, 0, 0, 0};
+        }
+    }
+    const int scales_at = L::TOKENS + eights * A.kb * 1024, fours = (eights + 1) >> 1;   // fours: 16-token columns
+    const int blocks = (A.rows + 127) >> 7;
+    if constexpr (is_f8(KIND)) {
+        for (int j = 0; j < fours; ++j) {
+            const float * src = A.bs + token_row(16 * j + (lane >> 2)) * A.kb;
+            for (int c = wave; 4 * c < A.kb; c += W) {
+                const int kb = 4 * c + (lane & 3);
+                load_to_lds_4(src + (kb < A.kb ? kb : A.kb - 1), lds0 + scales_at + (c * fours + j) * 256, -1);
+            }
+        }
+        for (int i = wave; i < L::BLOCKS; i += W) {
+            const int block = (n0 >> 7) + i < blocks ? (n0 >> 7) + i : blocks - 1;
+            load_to_lds_4(A.ws + (static_cast<int64_t>(t.group) * blocks + block) * A.kb + (lane < A.kb ? lane : A.kb - 1), lds0 + L::BLOCK_SCALES + i * 256, -1);
+        }
+    }
+    float * bias = reinterpret_cast<float *>(lds + L::BIAS);
+    for (int i = threadIdx.x; i < W * 16 * tiles; i += W * 64)
+        bias[i] = A.bias && n0 + i < A.rows ? A.bias[static_cast<int64_t>(t.group) * A.rows + n0 + i] : 0.0f;
+    int64_t to[L::NT];                                       // dst rows of token 16 j + r; -1: none
+    bool bad[L::NT];
+#pragma unroll
+    for (int j = 0; j < L::NT; ++j) {
+        const int64_t i = t.first + 16 * j + r;
+        to[j] = i < t.last ? target_row(A, i) : -1;
+        bad[j] = to[j] >= 0 && source_row(A, i) < 0;
+    }
+    landed<0>();
+    __syncthreads();
+
+    auto run = [&](auto t8_c) __attribute__((always_inline)) {
+        constexpr int T8 = decltype(t8_c)::value, NT = (T8 + 1) / 2;
+        const uint8_t * ring = lds + wave * (D * 2048);
+        int slot = 0;
+        for (int i = 0; i < my_tiles; ++i) {
+            const int n = (first_tile + W * i) * 16;
+            const float * wscale = reinterpret_cast<const float *>(lds + L::BLOCK_SCALES + ((n >> 7) - (n0 >> 7)) * 256);
+            f32x4 acc[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int kb = 0; kb < A.kb; ++kb) {
+                landed<(D - 1) * 2>();
+                const int left = A.k_bytes - kb * 128 - 32 * q;   // bytes of the row from this lane's pieces on
+                auto operand = [&](const uint8_t * rows, int rr, bool weights) __attribute__((always_inline)) {
+                    const uint8_t * p = rows + rr % 8 * 128;
+                    Piece v{*reinterpret_cast<const u32x4p *>(p + ((2 * q) ^ (rr >> 1)) * 16), *reinterpret_cast<const u32x4p *>(p + ((2 * q + 1) ^ (rr >> 1)) * 16)};
+                    if (weights && left < 32) {
+                        if (left <= 16) v.hi = u32x4p{0, 0, 0, 0};
+                        if (left <= 0) v.lo = u32x4p{0, 0, 0, 0};
+                    }
+                    Operand<KIND> o;
+                    o.take(v);
+                    return o;
+                };
+                const Operand<KIND> a = operand(ring + slot * 2048 + (r >> 3) * 1024, r, true);
+                float sw = 0.0f;
+                if constexpr (is_f8(KIND)) sw = wscale[kb];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    // (of eight tokens rows 8 .. 15 read rows 0 .. 7: their columns are not used)
+                    const int rr = 2 * j + 1 == T8 ? r & 7 : r;
+                    const Operand<KIND> b = operand(lds + L::TOKENS + ((2 * j + (rr >> 3)) * A.kb + kb) * 1024, rr, false);
+                    if constexpr (is_f8(KIND)) {
+                        const f32x4 p = product<KIND>(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        const float f = sw * *reinterpret_cast<const float *>(lds + scales_at + ((kb >> 2) * fours + j) * 256 + r * 16 + (kb & 3) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[j][e] = __builtin_fmaf(p[e], f, acc[j][e]);
+                    } else {
+                        acc[j] = product<KIND>(a, b, acc[j]);
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
+                issue();
+                slot = slot + 1 == D ? 0 : slot + 1;
+            }
+            const f32x4 extra = *reinterpret_cast<const f32x4 *>(bias + (n - n0) + 4 * q);
+            const float nan = __builtin_nanf("");
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if (to[j] >= 0 && n + 4 * q < A.rows) store4(A, to[j], n + 4 * q, bad[j] ? f32x4{nan, nan, nan, nan} : acc[j] + extra);
+        }
+        landed<0>();                                         // no load may land after the workgroup has ended
+    };
+    if constexpr (MAX8 >= 4) {
+        if (eights > 3) return run(std::integral_constant<int, 4>{});
+        if (eights > 2) return run(std::integral_constant<int, 3>{});
+    }
+    if constexpr (MAX8 >= 2) {
+        if (eights > 1) return run(std::integral_constant<int, 2>{});
+    }
+    run(std::integral_constant<int, 1>{});
+}
+
+// ----------------------------------------------------------------------------------- many tokens
 // Sixteen tokens' outputs from n on, fp32 in LDS (`row_bytes` a token), to their dst rows: PIECES of N values a token.
 template <int PIECES, int N>
 __device__ __forceinline__ void store_column(const ProductArgs & A, const uint8_t * from, int row_bytes, const int64_t * rows, int n) {
@@ -673,13 +897,28 @@ int64_t most_token_tiles(const ProductArgs & a, int tile_rows) {
     return a.offsets ? std::min(a.n_rows, a.n_rows / tile_rows + a.n_groups) : whole;
 }
 
-template <int KIND, int NT, int RS, int W>
+template <int KIND, int MAX8, int RS, int D>
 void launch_few_rows(const ProductArgs & a, hipStream_t stream) {
-    const int64_t row_tiles = (a.rows + 16 * RS - 1) / (16 * RS), blocks = row_tiles * most_token_tiles(a, 16 * NT);
-    require(blocks < (int64_t{1} << 32) / (W * 64), "too many outputs for one launch");
-    hipLaunchKernelGGL((few_rows_kernel<KIND, NT, RS, W>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, stream, a,
+    const int64_t row_tiles = (a.rows + 16 * RS - 1) / (16 * RS), blocks = row_tiles * most_token_tiles(a, 8 * MAX8);
+    require(blocks < (int64_t{1} << 24), "too many outputs for one launch");
+    hipLaunchKernelGGL((few_rows_kernel<KIND, MAX8, RS, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a,
                        static_cast<int>(row_tiles));
     check_hip(hipGetLastError(), "product launch");
+}
+
+// False: the tokens do not fit in LDS.
+template <int KIND, int MAX8, int W, int D>
+bool launch_stream_rows(const ProductArgs & a, int64_t groups, hipStream_t stream) {
+    using L = StreamLayout<KIND, MAX8, W, D>;
+    if (a.kb > L::MAX_KB) return false;
+    const int64_t row_tiles = (a.rows + 15) / 16;
+    const int tiles = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(L::MAX_TILES, groups * row_tiles / 4096)));
+    const int64_t units = (row_tiles + W * tiles - 1) / (W * tiles), blocks = units * most_token_tiles(a, 8 * MAX8);
+    require(blocks < (int64_t{1} << 32) / (W * 64), "too many outputs for one launch");
+    hipLaunchKernelGGL((stream_rows_kernel<KIND, MAX8, W, D>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, stream, a,
+                       static_cast<int>(units), tiles);
+    check_hip(hipGetLastError(), "product launch");
+    return true;
 }
 
 template <int KIND, int SN, int ST, int WN, int WT, int STAGES>
@@ -695,9 +934,17 @@ void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
 template <int KIND>
 void launch_product(const ProductArgs & a, hipStream_t stream) {
     const int64_t groups = std::min<int64_t>(a.n_groups, a.n_rows), mean = a.n_rows / groups;
-    if (mean <= 16) return launch_few_rows<KIND == kF8 ? kF8Wide : KIND, 1, 1, 4>(a, stream);
+    if (mean <= 16) {
+        const bool wide = groups * ((a.rows + 15) / 16) >= 4096;
+        if (mean <= 4) {
+            if (wide && (launch_stream_rows<KIND, 1, 4, 4>(a, groups, stream) || launch_stream_rows<KIND, 1, 8, 4>(a, groups, stream))) return;
+            return launch_few_rows<KIND, 1, 1, 4>(a, stream);
+        }
+        if (wide && (launch_stream_rows<KIND, 2, 4, 3>(a, groups, stream) || launch_stream_rows<KIND, 2, 8, 4>(a, groups, stream))) return;
+        return launch_few_rows<KIND, 2, 1, 3>(a, stream);
+    }
     auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
-    if (mean <= 32) launch_few_rows<KIND == kF8 ? kF8Wide : KIND, 4, 2, 4>(a, stream);
+    if (mean <= 32) launch_few_rows<KIND, 4, 2, 3>(a, stream);
     else if (KIND != kF8Wide && tiles(256, 256) >= 192) launch_many_rows<KIND == kF8Wide ? kF8 : KIND, 4, 8, 4, 2, 2>(a, stream);
     else if (tiles(128, 128) >= 192) launch_many_rows<KIND, 4, 4, 2, 2, 2>(a, stream);
     else launch_many_rows<KIND, 2, 2, 2, 2, 3>(a, stream);
