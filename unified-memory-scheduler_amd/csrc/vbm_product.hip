@@ -195,10 +195,14 @@ __device__ __forceinline__ f32x4 product(const Operand<KIND> & a, const Operand<
 __device__ __forceinline__ void load_to_lds_16(const void * src, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
 }
+// (with `some` and `lanes` none of a wave's, the load counts as one and brings nothing; all lanes are active where it is called)
+__device__ __forceinline__ void load_to_lds_16(const void * src, uint32_t m0, bool some, int lanes) {
+    if (!some) return load_to_lds_16(src, m0);
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dwordx4 %0, off\n\ts_mov_b64 exec, -1" ::"v"(src), "s"(m0), "s"(lanes) : "memory", "m0");
+}
 __device__ __forceinline__ void load_to_lds_16(const void * base, uint32_t offset, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(base), "v"(offset), "s"(m0) : "memory", "m0");
 }
-// (with `lanes` none of a wave's, the load counts as one and brings nothing; all lanes are active where it is called)
 __device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0, int lanes) {
     asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1" ::"v"(src), "s"(m0), "s"(lanes) : "memory", "m0");
 }
@@ -231,8 +235,9 @@ __device__ __forceinline__ void drain(int i, int n, const F & compute) {
 // are on their way. Each wave streams its own through a ring of D steps in LDS, without barriers: a load brings 128
 // bytes of each of eight rows, in neighbouring lanes (loaded straight into a matrix operand's registers, 16 rows in neighbouring lanes,
 // a kilobyte occupies the address unit for 64 cycles instead of 18, which alone limits a CU to 16 bytes a cycle).
-template <int KIND, int MAX8, int RS, int D>
+template <int KIND, int MAX8, int D>
 __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_tiles) {
+    constexpr int RS = 1;
     constexpr int W = 4, NT_MAX = (MAX8 + 1) / 2, RUN = 16;  // RUN: steps whose scales a wave holds
     constexpr int STEP = (2 * RS + MAX8) * 1024, SCALES = is_f8(KIND) ? RUN * 64 * NT_MAX : 0, WAVE = D * STEP + SCALES;
     static_assert(W * RS * NT_MAX * 1024 <= W * WAVE, "the ring's memory holds the waves' sums");
@@ -661,16 +666,15 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 }
 
 // A workgroup of WN x WT waves takes BN = 16 SN WN weight rows x up to BT = 16 ST WT tokens of one group; a wave 16 SN rows x every WT-th
-// 16-token column. A step's 128 bytes of every row are staged in LDS, STAGES - 1 steps ahead, with one wait and one barrier a
+// 16-token column. A step's 128 bytes of every row are staged in LDS, as many stages as the live columns leave room for, with one wait and one barrier a
 // step. Piece p (16 bytes) of row r lies at place p ^ (r / 2 % 8) of the row's 128 bytes, so that sixteen rows' reads of one piece
 // cover all 64 banks once (with p ^ (r % 8) rows r and r + 8 met in the same ones, and every read took twice as long).
-template <int KIND, int SN, int ST, int WN, int WT, int STAGES>
+template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
     constexpr int DW = BN / 8 / W, DT = BT / 8 / W;          // a wave's loads a step: 8 rows each
-    static_assert(DW * 8 * W == BN && DT * 8 * W == BT && BT % 64 == 0, "the waves share the loads evenly");
-    constexpr int STAGE = (BN + BT) * 128 + (is_f8(KIND) ? BT * 4 : 0);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
+    static_assert(DW * 8 * W == BN && DT * 8 * W == BT && BT % 32 == 0, "the waves share the loads evenly");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
     Work work;
     if (!find_work(A, ST * WT, row_tiles, work)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -695,8 +699,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     };
 #pragma unroll
     for (int i = 0; i < DT; ++i) tsrc[i] = A.b + token_row(8 * (wave + W * i) + (lane >> 3)) * A.k_bytes + piece * 16;
-    const int scale_slot = wave % (BT / 64);                 // the first BT / 64 waves bring the tokens' scales
-    const int scale_lanes = (wave - BT / 64) >> 31;
+    const int scale_slot = wave % ((BT + 63) / 64);
     const float * ssrc = nullptr, * wscale = nullptr;
     if constexpr (is_f8(KIND)) {
         ssrc = A.bs + token_row(64 * scale_slot + lane) * A.kb;
@@ -707,8 +710,12 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     const int live_cols = (work.live + 15) >> 4;
     auto run = [&](auto live_c) __attribute__((always_inline)) {
         constexpr int NT = decltype(live_c)::value;
-        constexpr int LOADS = DW + (NT * WT * 2 + W - 1) / W;                 // only the live columns' tokens
-        constexpr int PARTS = LOADS + (is_f8(KIND) ? 1 : 0);
+        constexpr int EIGHTS = NT * WT * 2, LOADS = DW + (EIGHTS + W - 1) / W;   // only the live columns' tokens
+        constexpr int PARTS = LOADS + (is_f8(KIND) ? 1 : 0), SCALE_WAVES = (EIGHTS + 7) / 8;
+        constexpr int SCALES = (BN + 8 * EIGHTS) * 128, STAGE = SCALES + (is_f8(KIND) ? SCALE_WAVES * 256 : 0);
+        constexpr int STAGES = LDS / STAGE < 4 ? LDS / STAGE : 4;
+        static_assert(STAGES >= 2 && SCALE_WAVES <= W, "two stages at least");
+        const int scale_lanes = (wave - SCALE_WAVES) >> 31;  // the first waves bring the tokens' scales
         f32x4 acc[SN][NT];
 #pragma unroll
         for (int s = 0; s < SN; ++s)
@@ -732,8 +739,9 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
 #pragma unroll
             for (int i = begin; i < end; ++i) {
                 if (i < DW) load_to_lds_16(wbase + off, wsrc[i < DW ? i : 0] + back, at + (wave + W * i) * 1024);
-                else if (i < LOADS) load_to_lds_16(tsrc[i - DW < DT ? i - DW : 0] + off + back, at + BN * 128 + (wave + W * (i - DW)) * 1024);
-                else load_to_lds_4(ssrc + kb, at + (BN + BT) * 128 + scale_slot * 256, scale_lanes);
+                else if (i < LOADS) load_to_lds_16(tsrc[i - DW < DT ? i - DW : 0] + off + back, at + BN * 128 + (wave + W * (i - DW)) * 1024,
+                                                   (i - DW + 1) * W > EIGHTS, (wave + W * (i - DW) - EIGHTS) >> 31);
+                else load_to_lds_4(ssrc + kb, at + SCALES + scale_slot * 256, scale_lanes);
             }
         };
 #pragma unroll
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
             const uint32_t stage = (kb % STAGES) * STAGE;
             a_lo = stage + 2048 * SN * wn + lo, a_hi = stage + 2048 * SN * wn + hi;
             b_lo = stage + BN * 128 + 2048 * wt + lo, b_hi = stage + BN * 128 + 2048 * wt + hi;
-            b_scale = stage + (BN + BT) * 128 + 64 * wt + 4 * r;
+            b_scale = stage + SCALES + 64 * wt + 4 * r;
             asm volatile("" : "+v"(a_lo), "+v"(a_hi), "+v"(b_lo), "+v"(b_hi), "+v"(b_scale));   // (offsets then fit the reads' own)
         };
         auto operand = [&](uint32_t at_lo, uint32_t at_hi, int rows) __attribute__((always_inline)) {
@@ -834,7 +842,8 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
 #pragma unroll
                 for (int i = 0; i < DW; ++i) *reinterpret_cast<u32x4p *>(mine + W * i * 1024) = u32x4p{0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < LOADS - DW; ++i) *reinterpret_cast<u32x4p *>(mine + BN * 128 + W * i * 1024) = u32x4p{0, 0, 0, 0};
+                for (int i = 0; i < LOADS - DW; ++i)
+                    if (wave + W * i < EIGHTS) *reinterpret_cast<u32x4p *>(mine + BN * 128 + W * i * 1024) = u32x4p{0, 0, 0, 0};
             }
             meet<0>();
             first_operands(whole);
@@ -850,7 +859,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         // A wave's 16-token column at a time goes through LDS, so that neighbouring lanes store neighbouring bytes of a dst row:
         // straight from the registers (16 rows x 32 bytes a store) the stores of a 4096 x 4096 output took 6 us longer.
         constexpr int ROW = 16 * SN * 4 + 16;                // bytes of a token's outputs there
-        static_assert(W * 16 * ROW + BT * 8 <= STAGES * STAGE, "the stages' memory holds them");
+        static_assert(W * 16 * ROW + BT * 8 <= LDS, "the stages' memory holds them");
         int64_t * rows = reinterpret_cast<int64_t *>(lds + W * 16 * ROW);   // dst row, -1: none, -2 - row: all NaN
         for (int c = threadIdx.x; c < BT; c += W * 64) {
             const int64_t i = static_cast<int64_t>(work.first) + c, row = c < work.live ? target_row(A, i) : -1;
@@ -897,11 +906,11 @@ int64_t most_token_tiles(const ProductArgs & a, int tile_rows) {
     return a.offsets ? std::min(a.n_rows, a.n_rows / tile_rows + a.n_groups) : whole;
 }
 
-template <int KIND, int MAX8, int RS, int D>
+template <int KIND, int MAX8, int D>
 void launch_few_rows(const ProductArgs & a, hipStream_t stream) {
-    const int64_t row_tiles = (a.rows + 16 * RS - 1) / (16 * RS), blocks = row_tiles * most_token_tiles(a, 8 * MAX8);
+    const int64_t row_tiles = (a.rows + 15) / 16, blocks = row_tiles * most_token_tiles(a, 8 * MAX8);
     require(blocks < (int64_t{1} << 24), "too many outputs for one launch");
-    hipLaunchKernelGGL((few_rows_kernel<KIND, MAX8, RS, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a,
+    hipLaunchKernelGGL((few_rows_kernel<KIND, MAX8, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a,
                        static_cast<int>(row_tiles));
     check_hip(hipGetLastError(), "product launch");
 }
@@ -921,12 +930,12 @@ bool launch_stream_rows(const ProductArgs & a, int64_t groups, hipStream_t strea
     return true;
 }
 
-template <int KIND, int SN, int ST, int WN, int WT, int STAGES>
+template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
     constexpr int BN = 16 * SN * WN, BT = 16 * ST * WT;
     const int64_t row_tiles = (a.rows + BN - 1) / BN, items = row_tiles * most_token_tiles(a, BT);
     require(items < (int64_t{1} << 32) / (WN * WT * 64) - 8, "too many outputs for one launch");
-    hipLaunchKernelGGL((many_rows_kernel<KIND, SN, ST, WN, WT, STAGES>), dim3(static_cast<unsigned>((items + 7) / 8 * 8)),
+    hipLaunchKernelGGL((many_rows_kernel<KIND, SN, ST, WN, WT, LDS>), dim3(static_cast<unsigned>((items + 7) / 8 * 8)),
                        dim3(WN * WT * 64), 0, stream, a, static_cast<int>(row_tiles));
     check_hip(hipGetLastError(), "product launch");
 }
@@ -934,20 +943,24 @@ void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
 template <int KIND>
 void launch_product(const ProductArgs & a, hipStream_t stream) {
     const int64_t groups = std::min<int64_t>(a.n_groups, a.n_rows), mean = a.n_rows / groups;
-    if (mean <= 16) {
+    if (mean <= 10) {
         const bool wide = groups * ((a.rows + 15) / 16) >= 4096;
         if (mean <= 4) {
             if (wide && (launch_stream_rows<KIND, 1, 4, 4>(a, groups, stream) || launch_stream_rows<KIND, 1, 8, 4>(a, groups, stream))) return;
-            return launch_few_rows<KIND, 1, 1, 4>(a, stream);
+            return launch_few_rows<KIND, 1, 4>(a, stream);
         }
         if (wide && (launch_stream_rows<KIND, 2, 4, 3>(a, groups, stream) || launch_stream_rows<KIND, 2, 8, 4>(a, groups, stream))) return;
-        return launch_few_rows<KIND, 2, 1, 3>(a, stream);
+        return launch_few_rows<KIND, 2, 3>(a, stream);
     }
     auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
-    if (mean <= 32) launch_few_rows<KIND, 4, 2, 3>(a, stream);
-    else if (KIND != kF8Wide && tiles(256, 256) >= 192) launch_many_rows<KIND == kF8Wide ? kF8 : KIND, 4, 8, 4, 2, 2>(a, stream);
-    else if (tiles(128, 128) >= 192) launch_many_rows<KIND, 4, 4, 2, 2, 2>(a, stream);
-    else launch_many_rows<KIND, 2, 2, 2, 2, 3>(a, stream);
+    if (mean > 40) {
+        if constexpr (KIND != kF8Wide) {                     // (widened operands do not leave it the registers)
+            if (tiles(256, 256) >= 160) return launch_many_rows<KIND, 4, 8, 4, 2, 160 * 1024>(a, stream);
+        }
+        if (tiles(256, 128) >= 140) return launch_many_rows<KIND, 2, 8, 8, 1, 160 * 1024>(a, stream);
+    }
+    if (tiles(128, 64) >= 160) return launch_many_rows<KIND, 2, 4, 4, 1, 80 * 1024>(a, stream);
+    launch_many_rows<KIND, 1, 2, 4, 1, 40 * 1024>(a, stream);
 }
 
 void product(const vbm_weights & w, const void * b, const float * b_scales, ProductArgs a, int dst_type, void * dst, hipStream_t stream) {
