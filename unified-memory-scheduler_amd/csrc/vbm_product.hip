@@ -563,7 +563,7 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
 // ----------------------------------------------------------------------------------- many tokens
 // Sixteen tokens' outputs from n on, fp32 in LDS (`row_bytes` a token), to their dst rows: PIECES of N values a token.
 template <int PIECES, int N>
-__device__ __forceinline__ void store_column(const ProductArgs & A, const uint8_t * from, int row_bytes, const int64_t * rows, int n) {
+__device__ __forceinline__ void store_column(const ProductArgs & A, const uint8_t * from, int row_bytes, const int * rows, int n) {
     constexpr int AT_ONCE = 64 / PIECES;                     // tokens
     const int lane = threadIdx.x & 63, at = n + lane % PIECES * N;
 #pragma unroll
@@ -624,12 +624,27 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
     auto bounded = [&](int v) { return v < 0 ? 0 : (v > n_rows ? n_rows : v); };
     auto columns = [&](int lo, int hi) { return hi > lo ? (hi - lo + 15) >> 4 : 0; };
     auto tiles_of = [&](int cols) { return (cols + most - 1) / most; };
+    // 64 groups a pass; the first passes' bounds stay in registers, so that their loads are on their way together
+    constexpr int KEPT = 4;
+    int kept_lo[KEPT], kept_hi[KEPT];
+    auto load = [&](int g, int & lo, int & hi) {
+        lo = g < A.n_groups ? bounded(A.offsets[g]) : 0;
+        hi = g < A.n_groups ? bounded(A.offsets[g + 1]) : 0;
+    };
     int total = 0;
     if (!A.offsets) {
         total = tiles_of(columns(0, n_rows));
     } else {
         int mine = 0;
-        for (int g = lane; g < A.n_groups; g += 64) mine += tiles_of(columns(bounded(A.offsets[g]), bounded(A.offsets[g + 1])));
+#pragma unroll
+        for (int c = 0; c < KEPT; ++c) load(64 * c + lane, kept_lo[c], kept_hi[c]);
+#pragma unroll
+        for (int c = 0; c < KEPT; ++c) mine += tiles_of(columns(kept_lo[c], kept_hi[c]));
+        for (int g = 64 * KEPT + lane; g < A.n_groups; g += 64) {
+            int lo, hi;
+            load(g, lo, hi);
+            mine += tiles_of(columns(lo, hi));
+        }
         total = __builtin_amdgcn_readlane(wave_inclusive_sum(mine), 63);
     }
     const int items = total * row_tiles, per_xcd = (items + 7) >> 3, slot = static_cast<int>(blockIdx.x >> 3);
@@ -640,21 +655,27 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
     w.group = 0;
     if (A.offsets) {
         int sum = 0;
-        for (int g0 = 0; g0 < A.n_groups; g0 += 64) {
-            const int g = g0 + lane;
-            const int l = g < A.n_groups ? bounded(A.offsets[g]) : 0, h = g < A.n_groups ? bounded(A.offsets[g + 1]) : 0;
+        auto holds = [&](int g0, int l, int h) {             // whether `index` is among these 64 groups' tiles
             const int t = tiles_of(columns(l, h)), incl = sum + wave_inclusive_sum(t);
             const uint64_t past = __ballot(incl > index);
-            if (past) {
-                const int who = __builtin_ctzll(past);
-                w.group = g0 + who;
-                lo = __builtin_amdgcn_readlane(l, who);
-                hi = __builtin_amdgcn_readlane(h, who);
-                tiles = __builtin_amdgcn_readlane(t, who);
-                before = __builtin_amdgcn_readlane(incl, who) - tiles;
-                break;
-            }
             sum = __builtin_amdgcn_readlane(incl, 63);
+            if (!past) return false;
+            const int who = __builtin_ctzll(past);
+            w.group = g0 + who;
+            lo = __builtin_amdgcn_readlane(l, who);
+            hi = __builtin_amdgcn_readlane(h, who);
+            tiles = __builtin_amdgcn_readlane(t, who);
+            before = __builtin_amdgcn_readlane(incl, who) - tiles;
+            return true;
+        };
+        bool found = false;
+#pragma unroll
+        for (int c = 0; c < KEPT; ++c)
+            if (!found) found = holds(64 * c, kept_lo[c], kept_hi[c]);
+        for (int g0 = 64 * KEPT; !found && g0 < A.n_groups; g0 += 64) {
+            int l, h;
+            load(g0 + lane, l, h);
+            found = holds(g0, l, h);
         }
     }
     const int local = item - before * row_tiles;
@@ -672,8 +693,9 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
-    constexpr int DW = BN / 8 / W, DT = BT / 8 / W;          // a wave's loads a step: 8 rows each
-    static_assert(DW * 8 * W == BN && DT * 8 * W == BT && BT % 32 == 0, "the waves share the loads evenly");
+    constexpr int DW = BN / 8 / W, DT = (BT / 8 + W - 1) / W;  // a wave's loads a step: 8 rows each
+    static_assert(DW * 8 * W == BN && BT % 32 == 0, "the waves share the loads");
+    constexpr int STAGE_BYTES = LDS - BT * 4;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
     Work work;
     if (!find_work(A, ST * WT, row_tiles, work)) return;
@@ -707,13 +729,20 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         wscale = A.ws + (static_cast<int64_t>(work.group) * (last + 1) + (block < last ? block : last)) * A.kb;
     }
 
+    int * rows = reinterpret_cast<int *>(lds + STAGE_BYTES);   // the tokens' dst rows, -1: none, -2 - row: all NaN
+    for (int c = threadIdx.x; c < BT; c += W * 64) {
+        const int64_t i = static_cast<int64_t>(work.first) + c;
+        const int row = c < work.live ? static_cast<int>(target_row(A, i)) : -1;
+        rows[c] = row >= 0 && source_row(A, i) < 0 ? -2 - row : row;
+    }
+
     const int live_cols = (work.live + 15) >> 4;
     auto run = [&](auto live_c) __attribute__((always_inline)) {
         constexpr int NT = decltype(live_c)::value;
         constexpr int EIGHTS = NT * WT * 2, LOADS = DW + (EIGHTS + W - 1) / W;   // only the live columns' tokens
         constexpr int PARTS = LOADS + (is_f8(KIND) ? 1 : 0), SCALE_WAVES = (EIGHTS + 7) / 8;
         constexpr int SCALES = (BN + 8 * EIGHTS) * 128, STAGE = SCALES + (is_f8(KIND) ? SCALE_WAVES * 256 : 0);
-        constexpr int STAGES = LDS / STAGE < 4 ? LDS / STAGE : 4;
+        constexpr int STAGES = STAGE_BYTES / STAGE < 4 ? STAGE_BYTES / STAGE : 4;
         static_assert(STAGES >= 2 && SCALE_WAVES <= W, "two stages at least");
         const int scale_lanes = (wave - SCALE_WAVES) >> 31;  // the first waves bring the tokens' scales
         f32x4 acc[SN][NT];
@@ -859,13 +888,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         // A wave's 16-token column at a time goes through LDS, so that neighbouring lanes store neighbouring bytes of a dst row:
         // straight from the registers (16 rows x 32 bytes a store) the stores of a 4096 x 4096 output took 6 us longer.
         constexpr int ROW = 16 * SN * 4 + 16;                // bytes of a token's outputs there
-        static_assert(W * 16 * ROW + BT * 8 <= LDS, "the stages' memory holds them");
-        int64_t * rows = reinterpret_cast<int64_t *>(lds + W * 16 * ROW);   // dst row, -1: none, -2 - row: all NaN
-        for (int c = threadIdx.x; c < BT; c += W * 64) {
-            const int64_t i = static_cast<int64_t>(work.first) + c, row = c < work.live ? target_row(A, i) : -1;
-            rows[c] = row >= 0 && source_row(A, i) < 0 ? -2 - row : row;
-        }
-        __syncthreads();
+        static_assert(W * 16 * ROW <= STAGE_BYTES, "the stages' memory holds them");
         const int nw = n0 + 16 * SN * wn;                    // the wave's first output
         f32x4 bias[SN];
 #pragma unroll
@@ -880,7 +903,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
             for (int s = 0; s < SN; ++s) *reinterpret_cast<f32x4 *>(mine + r * ROW + 64 * s + 16 * q) = acc[s][j] + bias[s];
-            const int64_t * to = rows + 16 * (j * WT + wt);
+            const int * to = rows + 16 * (j * WT + wt);
             if (A.dst_type == VBM_TYPE_F32) store_column<4 * SN, 4>(A, mine, ROW, to, nw);
             else store_column<2 * SN, 8>(A, mine, ROW, to, nw);
         }
@@ -889,7 +912,11 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     const int nt = (live_cols + WT - 1) / WT;
     if constexpr (ST >= 8) {
         if (nt > 6) return run(std::integral_constant<int, 8>{});
+    }
+    if constexpr (ST >= 6) {
         if (nt > 5) return run(std::integral_constant<int, 6>{});
+    }
+    if constexpr (ST >= 5) {
         if (nt > 4) return run(std::integral_constant<int, 5>{});
     }
     if constexpr (ST >= 4) {
@@ -955,6 +982,7 @@ void launch_product(const ProductArgs & a, hipStream_t stream) {
     auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
     if (mean > 40) {
         if constexpr (KIND != kF8Wide) {                     // (widened operands do not leave it the registers)
+            if (a.offsets && mean > 140 && tiles(256, 160) >= 160) return launch_many_rows<KIND, 4, 5, 4, 2, 160 * 1024>(a, stream);
             if (tiles(256, 256) >= 160) return launch_many_rows<KIND, 4, 8, 4, 2, 160 * 1024>(a, stream);
         }
         if (tiles(256, 128) >= 140) return launch_many_rows<KIND, 2, 8, 8, 1, 160 * 1024>(a, stream);
@@ -971,7 +999,7 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     require(w.rows > 0 && w.rows < (int64_t{1} << 30) && w.k > 0 && w.k < (int64_t{1} << 23), "rows and k out of range");
     const int64_t k_bytes = w.k * (f8 ? 1 : 2);
     require(k_bytes % 16 == 0, f8 ? "k must be a multiple of 16" : "k must be a multiple of 8");
-    require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 31) && a.n_b >= 0 && a.n_dst >= 0, "row counts out of range");
+    require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 31) && a.n_b >= 0 && a.n_dst >= 0 && a.n_dst < (int64_t{1} << 31) - 2, "row counts out of range");
     require(a.b_div > 0 && a.b_div < (int64_t{1} << 31), "b_div must be positive");
     if (a.n_rows == 0) return;
     require(w.data && b && dst && a.n_b > 0 && (!f8 || (w.scales && b_scales)), "null buffer");
