@@ -64,14 +64,59 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
     return v;
 }
 
+// The groups' bounds, 64 groups a pass, lane by lane; those of the first passes stay in registers, so that their loads are on
+// their way together. Offsets are bounded to [0, n_rows]: bad ones cannot lead out of the buffers.
+struct Groups {
+    static constexpr int KEPT = 4;
+    const ProductArgs & A;
+    int lo[KEPT], hi[KEPT];
+    __device__ __forceinline__ explicit Groups(const ProductArgs & args) : A(args) {
+#pragma unroll
+        for (int c = 0; c < KEPT; ++c) load(64 * c, lo[c], hi[c]);
+    }
+    __device__ __forceinline__ void load(int g0, int & l, int & h) const {
+        const int g = g0 + static_cast<int>(threadIdx.x & 63), n = static_cast<int>(A.n_rows);
+        auto bounded = [&](int v) { return v < 0 ? 0 : (v > n ? n : v); };
+        l = g < A.n_groups ? bounded(A.offsets[g]) : 0;
+        h = g < A.n_groups ? bounded(A.offsets[g + 1]) : 0;
+    }
+    // Calls f(g0, lo, hi) pass by pass, until it returns true.
+    template <class F>
+    __device__ __forceinline__ void each(F && f) const {
+        bool done = false;
+#pragma unroll
+        for (int c = 0; c < KEPT; ++c)
+            if (!done && 64 * c < A.n_groups) done = f(64 * c, lo[c], hi[c]);
+        for (int g0 = 64 * KEPT; !done && g0 < A.n_groups; g0 += 64) {
+            int l, h;
+            load(g0, l, h);
+            done = f(g0, l, h);
+        }
+    }
+};
+// Of tiles in group order, `t` of them in this lane's group of a pass: whether number `index` is in this pass, and its group's
+// lane, number of tiles and the tiles before it. `sum`: the tiles of earlier passes, brought up to date.
+struct Place {
+    int lane, tiles, before;
+};
+__device__ __forceinline__ bool find_place(int t, int index, int & sum, Place & p) {
+    const int incl = sum + wave_inclusive_sum(t);
+    const uint64_t past = __ballot(incl > index);
+    sum = __builtin_amdgcn_readlane(incl, 63);
+    if (!past) return false;
+    p.lane = __builtin_ctzll(past);
+    p.tiles = __builtin_amdgcn_readlane(t, p.lane);
+    p.before = __builtin_amdgcn_readlane(incl, p.lane) - p.tiles;
+    return true;
+}
+
 struct TokenTile {
     int group;
     int64_t first, last;           // grouped rows [first, last)
 };
 
-// The group and rows of token tile `index`, tiles of BT rows in group order; false past the last one. Every wave finds it
-// from the offsets by itself (the host does not know the groups' sizes, and a launch that wrote the list would cost more). Offsets
-// are bounded to [0, n_rows], so that bad ones cannot lead out of the buffers.
+// The group and rows of token tile `index`, tiles of `tile_rows` in group order; false past the last one. Every wave finds it
+// from the offsets by itself (the host does not know the groups' sizes, and a launch that wrote the list would cost more).
 __device__ __forceinline__ bool find_token_tile(const ProductArgs & A, int index, int tile_rows, TokenTile & t) {
     if (!A.offsets) {
         t.group = 0;
@@ -79,28 +124,19 @@ __device__ __forceinline__ bool find_token_tile(const ProductArgs & A, int index
         t.last = t.first + tile_rows < A.n_rows ? t.first + tile_rows : A.n_rows;
         return t.first < A.n_rows;
     }
-    const int lane = threadIdx.x & 63;
-    const int n_rows = static_cast<int>(A.n_rows);
-    auto bounded = [&](int v) { return v < 0 ? 0 : (v > n_rows ? n_rows : v); };
-    int before = 0;
-    for (int g0 = 0; g0 < A.n_groups; g0 += 64) {
-        const int g = g0 + lane;
-        const bool live = g < A.n_groups;
-        const int lo = live ? bounded(A.offsets[g]) : 0, hi = live ? bounded(A.offsets[g + 1]) : 0;
-        const int tiles = hi > lo ? (hi - lo + tile_rows - 1) / tile_rows : 0;
-        const int incl = before + wave_inclusive_sum(tiles);
-        const uint64_t past = __ballot(incl > index);
-        if (past) {
-            const int who = __builtin_ctzll(past);
-            const int start = __shfl(lo, who) + (index - __shfl(incl - tiles, who)) * tile_rows, end = __shfl(hi, who);
-            t.group = __builtin_amdgcn_readfirstlane(g0 + who);
-            t.first = __builtin_amdgcn_readfirstlane(start);
-            t.last = __builtin_amdgcn_readfirstlane(start + tile_rows < end ? start + tile_rows : end);
-            return true;
-        }
-        before = __builtin_amdgcn_readlane(incl, 63);
-    }
-    return false;
+    const Groups groups(A);
+    int sum = 0;
+    bool found = false;
+    groups.each([&](int g0, int lo, int hi) {
+        Place p;
+        if (!find_place(hi > lo ? (hi - lo + tile_rows - 1) / tile_rows : 0, index, sum, p)) return false;
+        const int start = __builtin_amdgcn_readlane(lo, p.lane) + (index - p.before) * tile_rows, end = __builtin_amdgcn_readlane(hi, p.lane);
+        t.group = g0 + p.lane;
+        t.first = start;
+        t.last = start + tile_rows < end ? start + tile_rows : end;
+        return found = true;
+    });
+    return found;
 }
 
 // Grouped row i's row of b; -1: none (its outputs are NaN).
@@ -620,63 +656,38 @@ struct Work {
 // i % 8, so each XCD takes a contiguous run of the list (group by group, row tile by row tile): the token tiles that share a row
 // tile's weights, and the row tiles that share the tokens, then meet in one L2. A group's tiles share its columns evenly.
 __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int row_tiles, Work & w) {
-    const int lane = threadIdx.x & 63, n_rows = static_cast<int>(A.n_rows);
-    auto bounded = [&](int v) { return v < 0 ? 0 : (v > n_rows ? n_rows : v); };
+    const int n_rows = static_cast<int>(A.n_rows), slot = static_cast<int>(blockIdx.x >> 3);
     auto columns = [&](int lo, int hi) { return hi > lo ? (hi - lo + 15) >> 4 : 0; };
-    auto tiles_of = [&](int cols) { return (cols + most - 1) / most; };
-    // 64 groups a pass; the first passes' bounds stay in registers, so that their loads are on their way together
-    constexpr int KEPT = 4;
-    int kept_lo[KEPT], kept_hi[KEPT];
-    auto load = [&](int g, int & lo, int & hi) {
-        lo = g < A.n_groups ? bounded(A.offsets[g]) : 0;
-        hi = g < A.n_groups ? bounded(A.offsets[g + 1]) : 0;
+    auto tiles_of = [&](int lo, int hi) { return (columns(lo, hi) + most - 1) / most; };
+    int item = 0, lo = 0, hi = n_rows, tiles = 0, before = 0;
+    auto mine = [&](int total) {                             // this workgroup's item of so many token tiles
+        const int items = total * row_tiles, per_xcd = (items + 7) >> 3;
+        item = static_cast<int>(blockIdx.x & 7) * per_xcd + slot;
+        return slot < per_xcd && item < items;
     };
-    int total = 0;
-    if (!A.offsets) {
-        total = tiles_of(columns(0, n_rows));
-    } else {
-        int mine = 0;
-#pragma unroll
-        for (int c = 0; c < KEPT; ++c) load(64 * c + lane, kept_lo[c], kept_hi[c]);
-#pragma unroll
-        for (int c = 0; c < KEPT; ++c) mine += tiles_of(columns(kept_lo[c], kept_hi[c]));
-        for (int g = 64 * KEPT + lane; g < A.n_groups; g += 64) {
-            int lo, hi;
-            load(g, lo, hi);
-            mine += tiles_of(columns(lo, hi));
-        }
-        total = __builtin_amdgcn_readlane(wave_inclusive_sum(mine), 63);
-    }
-    const int items = total * row_tiles, per_xcd = (items + 7) >> 3, slot = static_cast<int>(blockIdx.x >> 3);
-    const int item = static_cast<int>(blockIdx.x & 7) * per_xcd + slot;
-    if (slot >= per_xcd || item >= items) return false;
-    const int index = item / row_tiles;
-    int lo = 0, hi = n_rows, tiles = total, before = 0;
     w.group = 0;
-    if (A.offsets) {
-        int sum = 0;
-        auto holds = [&](int g0, int l, int h) {             // whether `index` is among these 64 groups' tiles
-            const int t = tiles_of(columns(l, h)), incl = sum + wave_inclusive_sum(t);
-            const uint64_t past = __ballot(incl > index);
-            sum = __builtin_amdgcn_readlane(incl, 63);
-            if (!past) return false;
-            const int who = __builtin_ctzll(past);
-            w.group = g0 + who;
-            lo = __builtin_amdgcn_readlane(l, who);
-            hi = __builtin_amdgcn_readlane(h, who);
-            tiles = __builtin_amdgcn_readlane(t, who);
-            before = __builtin_amdgcn_readlane(incl, who) - tiles;
+    if (!A.offsets) {
+        tiles = tiles_of(0, n_rows);
+        if (!mine(tiles)) return false;
+    } else {
+        const Groups groups(A);
+        int part = 0, sum = 0;
+        groups.each([&](int, int l, int h) {
+            part += tiles_of(l, h);
+            return false;
+        });
+        if (!mine(__builtin_amdgcn_readlane(wave_inclusive_sum(part), 63))) return false;
+        const int index = item / row_tiles;
+        groups.each([&](int g0, int l, int h) {
+            Place p;
+            if (!find_place(tiles_of(l, h), index, sum, p)) return false;
+            w.group = g0 + p.lane;
+            lo = __builtin_amdgcn_readlane(l, p.lane);
+            hi = __builtin_amdgcn_readlane(h, p.lane);
+            tiles = p.tiles;
+            before = p.before;
             return true;
-        };
-        bool found = false;
-#pragma unroll
-        for (int c = 0; c < KEPT; ++c)
-            if (!found) found = holds(64 * c, kept_lo[c], kept_hi[c]);
-        for (int g0 = 64 * KEPT; !found && g0 < A.n_groups; g0 += 64) {
-            int l, h;
-            load(g0 + lane, l, h);
-            found = holds(g0, l, h);
-        }
+        });
     }
     const int local = item - before * row_tiles;
     w.row_tile = local / tiles;
