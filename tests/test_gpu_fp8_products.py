@@ -137,7 +137,8 @@ def test_glu_quantize_marks_blocks_without_a_scale(gpu):
 @pytest.mark.parametrize("dst_type", TYPES)
 @pytest.mark.parametrize("tokens,rows,k,bias", [(1, 64, 128, False), (1, 300, 2880, True), (2, 1, 16, True), (15, 129, 48, False), (16, 15, 144, False),
                                                 (17, 100, 336, True), (40, 130, 2048, False), (65, 257, 720, True), (130, 515, 400, False),
-                                                (300, 384, 1040, True), (2085, 6164, 144, True), (1000, 2000, 272, False)])
+                                                (300, 384, 1040, True), (2085, 6164, 144, True), (1000, 2000, 272, False),
+                                                (3, 70, 8720, True), (9, 33, 8832, False), (300, 130, 8720, True), (2500, 4100, 8336, False)])
 def test_dense_product(gpu, dst_type, tokens, rows, k, bias):
     rng = np.random.default_rng(tokens * 31 + rows)
     m, x = R.Matrix(F8, rng, 1, rows, k, bias), R.Tokens(F8, rng, tokens, k)
@@ -228,6 +229,37 @@ def test_grouped_product_many_rows(gpu, type_id, dst_type, gather, rows, k, grou
     kw = dict(b_rows=place, b_div=top_k) if gather else dict(dst_rows=place)
     got = R.grouped(m, x, n_b, offsets, n_rows, dst_type, n_rows, **kw)
     R.check(m, dst_type, got, *R.grouped_want(m, x, n_b, offsets, n_rows, n_rows, **kw), f"many rows {rows}x{k}")
+
+
+@pytest.mark.parametrize("dst_type,offset", [(F32, 4), (F32, 8), (F16, 2), (BF16, 6), (BF16, 8)])
+@pytest.mark.parametrize("tokens,rows", [(2, 64), (30, 72), (333, 256)])
+def test_outputs_that_are_aligned_to_their_type_only(gpu, dst_type, offset, tokens, rows):
+    rng = np.random.default_rng(offset + tokens)
+    k = 208
+    m, x = R.Matrix(F8, rng, 1, rows, k, True), R.Tokens(F8, rng, tokens, k)
+    size = R.SIZE[dst_type]
+    dst = R.filled(16 + tokens * rows * size + 64)
+    vb.call("vbm_mul_mat_fp8", m.desc, x.data.ptr, x.scales.ptr, tokens, dst_type, dst.ptr + offset, None)
+    sync()
+    raw = dst.download(np.uint8, (dst.nbytes,))
+    end = offset + tokens * rows * size
+    assert (raw[:offset] == R.FILL).all() and (raw[end:] == R.FILL).all()
+    out = raw[offset:end].copy()
+    got = {F32: lambda: out.view(np.float32), F16: lambda: out.view(np.float16), BF16: lambda: R.bf16_values(out.view(np.uint16))}[dst_type]()
+    y, mag, written = R.grouped_want(m, x, tokens, [0, tokens], tokens, tokens)
+    R.check(m, dst_type, got.astype(np.float64).reshape(tokens, rows), y, mag, written, "unaligned outputs")
+
+
+def test_a_call_gives_the_same_bits_again(gpu):
+    """Few, some and many rows a group: repeated calls, with other work between them, give equal bits."""
+    rng = np.random.default_rng(21)
+    for type_id, counts, rows, k in ((F8, [3, 1, 2], 100, 528), (F8, [60, 0, 33], 640, 1040), (BF16, [300, 200], 1100, 264), (F8, [9] * 70, 1000, 400)):
+        offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        n = int(offsets[-1])
+        m, x = R.Matrix(type_id, rng, len(counts), rows, k), R.Tokens(type_id, rng, n, k)
+        first = R.grouped(m, x, n, offsets, n, F32, n)
+        for _ in range(3):
+            assert np.array_equal(R.grouped(m, x, n, offsets, n, F32, n), first)
 
 
 @pytest.mark.parametrize("type_id", [F8, F16])
