@@ -11,7 +11,8 @@
 // or an infinity has no scale: it comes out as a NaN scale and zero codes, so that every product with it is NaN.
 //
 // Bound by bandwidth (one read of the inputs, one write of a quarter to half of them). Sixteen lanes share a block, eight values
-// each: 16- or 2 x 16-byte loads, an 8-byte store of codes, and the maximum over 16 lanes by four DPP moves.
+// each: 16- or 2 x 16-byte loads, an 8-byte store of codes, and the maximum over 16 lanes by four DPP moves. 8192 x 4096 bf16 19 to
+// 21 us (5.0 TB/s), GLU of 8192 x 2880 fp32 pairs 33 to 40 us (5.3 TB/s, where a large copy reaches 5.1); one row 2 us, a launch.
 #include <type_traits>
 
 #include "vbm_device.hpp"

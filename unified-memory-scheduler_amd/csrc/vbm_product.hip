@@ -271,6 +271,8 @@ __device__ __forceinline__ void drain(int i, int n, const F & compute) {
 // are on their way. Each wave streams its own through a ring of D steps in LDS, without barriers: a load brings 128
 // bytes of each of eight rows, in neighbouring lanes (loaded straight into a matrix operand's registers, 16 rows in neighbouring lanes,
 // a kilobyte occupies the address unit for 64 cycles instead of 18, which alone limits a CU to 16 bytes a cycle).
+// One token through eight FP8 experts of 1536 x 2048: 6.4 us, of which the 25 MB take 5 at the rate of a large copy; one token
+// through one matrix of 5760 x 2880: 5.9 us, latency: bounds and rows, the weights, the waves' sums.
 template <int KIND, int MAX8, int D>
 __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_tiles) {
     constexpr int RS = 1;
@@ -429,7 +431,9 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
 
 // The same where there are rows enough to keep the card busy with one wave a row tile: the tokens, of all of the depth, are staged in LDS
 // once and shared by the workgroup's W waves; then each wave streams `tiles` row tiles of 16 rows, one after the other through
-// a ring of D steps, with no barrier and no sums to join.
+// a ring of D steps, with no barrier and no sums to join. 64 tokens top-4 over 32 FP8 experts of 5760 x 2880, fp32 outputs: 106 us,
+// 5.05 TB/s (a large copy reaches 5.1); with the depth shared among the waves 134..163. 16 tokens top-4 over 32 bf16 experts of 2880 x
+// 2880: 82 us, 5.7 TB/s. Bound by memory.
 template <int KIND, int MAX8, int W, int D>
 struct StreamLayout {
     static constexpr int NT = (MAX8 + 1) / 2, MAX_TILES = 4;
@@ -698,9 +702,17 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 }
 
 // A workgroup of WN x WT waves takes BN = 16 SN WN weight rows x up to BT = 16 ST WT tokens of one group; a wave 16 SN rows x every WT-th
-// 16-token column. A step's 128 bytes of every row are staged in LDS, as many stages as the live columns leave room for, with one wait and one barrier a
-// step. Piece p (16 bytes) of row r lies at place p ^ (r / 2 % 8) of the row's 128 bytes, so that sixteen rows' reads of one piece
-// cover all 64 banks once (with p ^ (r % 8) rows r and r + 8 met in the same ones, and every read took twice as long).
+// 16-token column. A step's 128 bytes of every row are staged in LDS, as many stages as the live columns leave room for, with one
+// wait and one barrier a step. Piece p (16 bytes) of row r lies at place p ^ (r / 2 % 8) of the row's 128 bytes: sixteen rows'
+// reads of one piece then cover all banks (unswizzled they took twice as long).
+//
+// FP8 4096 x 4096 x 4096 with 16-bit outputs: 65 to 67 us, 2.1 PFLOP/s, where a library's product without block scales reaches 2.7.
+// Per step of 256 x 256 (1.75 us): the matrix instructions alone 1.0, with the fp32 sums of the scaled blocks 1.25 (an FMA per output and
+// block, half of a matrix instruction's time), the LDS reads under them; the rest is the loads' issue: a wave stands still until
+// the address unit has taken its kilobyte (18 cycles each, 64 of them a step), and the waves of a workgroup ask for it together.
+// What was tried: all of a step's loads at once 1.78; four-wave workgroups of 256 x 128 84 us; items dealt to the XCDs in turn, not in
+// runs: the same here, 5 % slower for ragged groups. Grouped prefill is bound by the weights' stream and what a workgroup
+// does not overlap with it: one of them fits a CU, and its start (bounds, rows, first stages) and end cost about 8 us of some 40.
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
@@ -978,8 +990,21 @@ void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
     check_hip(hipGetLastError(), "product launch");
 }
 
+// Which kernel, by the rows a group has on average and the tiles that a launch then has for 256 CUs (us, FP8 unless said otherwise):
+// - up to 10 rows: the streaming kernels. 32 experts of 5760 x 2880, 8 rows 107, 10 rows 108, 12 rows 114 and 16 rows 133, against 109, 111,
+//   112 and 115 in tiles of 128 x 64. Tokens by eights up to 4 rows: 16-bit experts of 2880 x 2880, 2 rows 82 against 85.
+//   One wave a row tile from 4096 row tiles on (two for each wave that the card holds); the depth shared among four
+//   waves below that.
+// - 11 to 40 rows: 128 x 64 (128 experts of 1536 x 2048: 16 rows 80, 32 rows 86, against 86 and 90 in tiles of 256 x 256; bf16, 32 experts of 2880 x
+//   2880, 16 rows 100 against 106), 64 x 32 where there are too few of those: 333 tokens x 2880 x 2880 13.9 against 15.4, 100 tokens 10.6
+//   against 15.0; but 700 tokens 23.2 against 16.4, 512 x 4096 x 4096 25.0 against 19.0.
+// - more: 256 x 256, or 256 x 128 where that leaves CUs idle: 2048 x 2880 x 2880 30 against 46, 2048 x 5760 x 2880 57.5 against 47; and 128 x 64 where
+//   that does too: 2048 x 2048 x 2048 18.9 against 22.0, 1500 x 2880 x 2880 34.5 against 28.8. Groups of more than 140 rows take two
+//   256 x 160 tiles rather than one 256 x 256, which leave LDS for a third stage: 256 rows, 2880 x 2880 137 against 153, bf16 5760 x
+//   2880 351 against 375; 140 rows 77 against 71. (kF8Wide: 256 x 256 would not leave it the registers.)
 template <int KIND>
 void launch_product(const ProductArgs & a, hipStream_t stream) {
+    if (a.n_rows == 0) return;
     const int64_t groups = std::min<int64_t>(a.n_groups, a.n_rows), mean = a.n_rows / groups;
     if (mean <= 10) {
         const bool wide = groups * ((a.rows + 15) / 16) >= 4096;
@@ -992,7 +1017,7 @@ void launch_product(const ProductArgs & a, hipStream_t stream) {
     }
     auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
     if (mean > 40) {
-        if constexpr (KIND != kF8Wide) {                     // (widened operands do not leave it the registers)
+        if constexpr (KIND != kF8Wide) {
             if (a.offsets && mean > 140 && tiles(256, 160) >= 160) return launch_many_rows<KIND, 4, 5, 4, 2, 160 * 1024>(a, stream);
             if (tiles(256, 256) >= 160) return launch_many_rows<KIND, 4, 8, 4, 2, 160 * 1024>(a, stream);
         }
