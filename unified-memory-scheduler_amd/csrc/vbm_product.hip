@@ -231,16 +231,15 @@ __device__ __forceinline__ f32x4 product(const Operand<KIND> & a, const Operand<
 __device__ __forceinline__ void load_to_lds_16(const void * src, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
 }
-// (with `some` and `lanes` none of a wave's, the load counts as one and brings nothing; all lanes are active where it is called)
-__device__ __forceinline__ void load_to_lds_16(const void * src, uint32_t m0, bool some, int lanes) {
-    if (!some) return load_to_lds_16(src, m0);
-    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dwordx4 %0, off\n\ts_mov_b64 exec, -1" ::"v"(src), "s"(m0), "s"(lanes) : "memory", "m0");
-}
 __device__ __forceinline__ void load_to_lds_16(const void * base, uint32_t offset, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(base), "v"(offset), "s"(m0) : "memory", "m0");
 }
-__device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0, int lanes) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1" ::"v"(src), "s"(m0), "s"(lanes) : "memory", "m0");
+__device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
+}
+// By all lanes (`all` -1) or by lane 0 alone (0), which the waits count alike; all lanes are active where it is called.
+__device__ __forceinline__ void load_to_lds_4(const void * src, uint32_t m0, int all) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1" ::"v"(src), "s"(m0), "s"(all | 1), "s"(all) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 // Waits until all but the wave's newest N loads have landed and its LDS reads are done, then for the workgroup's other waves.
@@ -329,7 +328,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         const int k = k0 + 4 * c + (lane & 3);
-                        load_to_lds_4(ssrc[j] + (k < A.kb ? k : A.kb - 1), lds0 + D * STEP + (c * NT_MAX + j) * 256, -1);
+                        load_to_lds_4(ssrc[j] + (k < A.kb ? k : A.kb - 1), lds0 + D * STEP + (c * NT_MAX + j) * 256);
                     }
             }
             auto issue = [&](int i) __attribute__((always_inline)) {
@@ -515,12 +514,12 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
             const float * src = A.bs + token_row(16 * j + (lane >> 2)) * A.kb;
             for (int c = wave; 4 * c < A.kb; c += W) {
                 const int kb = 4 * c + (lane & 3);
-                load_to_lds_4(src + (kb < A.kb ? kb : A.kb - 1), lds0 + scales_at + (c * fours + j) * 256, -1);
+                load_to_lds_4(src + (kb < A.kb ? kb : A.kb - 1), lds0 + scales_at + (c * fours + j) * 256);
             }
         }
         for (int i = wave; i < L::BLOCKS; i += W) {
             const int block = (n0 >> 7) + i < blocks ? (n0 >> 7) + i : blocks - 1;
-            load_to_lds_4(A.ws + (static_cast<int64_t>(t.group) * blocks + block) * A.kb + (lane < A.kb ? lane : A.kb - 1), lds0 + L::BLOCK_SCALES + i * 256, -1);
+            load_to_lds_4(A.ws + (static_cast<int64_t>(t.group) * blocks + block) * A.kb + (lane < A.kb ? lane : A.kb - 1), lds0 + L::BLOCK_SCALES + i * 256);
         }
     }
     float * bias = reinterpret_cast<float *>(lds + L::BIAS);
@@ -716,7 +715,7 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
-    constexpr int DW = BN / 8 / W, DT = (BT / 8 + W - 1) / W;  // a wave's loads a step: 8 rows each
+    constexpr int DW = BN / 8 / W;                           // a wave's loads of weights a step: 8 rows each
     static_assert(DW * 8 * W == BN && BT % 32 == 0, "the waves share the loads");
     constexpr int STAGE_BYTES = LDS - BT * 4;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
@@ -727,7 +726,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     const int n0 = work.row_tile * BN;
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
 
-    const uint8_t * wbase = A.w + (static_cast<int64_t>(work.group) * A.rows + n0) * A.k_bytes, * tsrc[DT];
+    const uint8_t * wbase = A.w + (static_cast<int64_t>(work.group) * A.rows + n0) * A.k_bytes;
     uint32_t wsrc[DW];                                       // (rows of a tile are at most 2^32 bytes apart)
     // the piece that this lane brings of row lane / 8 of eight: place lane % 8, of rows 0 .. 7 or 8 .. 15 of sixteen (loads k = wave + W i
     // with even or odd k; W is even, so all of a wave's are alike)
@@ -742,12 +741,8 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         const int64_t src = source_row(A, work.first + (i < work.live ? i : 0));
         return src < 0 ? 0 : src;
     };
-#pragma unroll
-    for (int i = 0; i < DT; ++i) tsrc[i] = A.b + token_row(8 * (wave + W * i) + (lane >> 3)) * A.k_bytes + piece * 16;
-    const int scale_slot = wave % ((BT + 63) / 64);
-    const float * ssrc = nullptr, * wscale = nullptr;
+    const float * wscale = nullptr;
     if constexpr (is_f8(KIND)) {
-        ssrc = A.bs + token_row(64 * scale_slot + lane) * A.kb;
         const int block = (n0 + 16 * SN * wn) >> 7, last = (A.rows - 1) >> 7;
         wscale = A.ws + (static_cast<int64_t>(work.group) * (last + 1) + (block < last ? block : last)) * A.kb;
     }
@@ -767,7 +762,19 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         constexpr int SCALES = (BN + 8 * EIGHTS) * 128, STAGE = SCALES + (is_f8(KIND) ? SCALE_WAVES * 256 : 0);
         constexpr int STAGES = STAGE_BYTES / STAGE < 4 ? STAGE_BYTES / STAGE : 4;
         static_assert(STAGES >= 2 && SCALE_WAVES <= W, "two stages at least");
-        const int scale_lanes = (wave - SCALE_WAVES) >> 31;  // the first waves bring the tokens' scales
+        // Every wave issues the same number of loads, which the waits count: past the live columns it loads eight tokens that another one
+        // loads too (of the same parity, so that the pieces' places agree); and the first waves bring the tokens' scales, the others
+        // one of the same.
+        const float * ssrc = is_f8(KIND) ? A.bs + token_row(64 * (wave % SCALE_WAVES) + lane) * A.kb : nullptr;
+        const int scale_lanes = (wave - SCALE_WAVES) >> 31;
+        const uint8_t * tsrc[LOADS - DW];
+        int place[LOADS - DW];
+#pragma unroll
+        for (int i = 0; i < LOADS - DW; ++i) {
+            const int eight = (wave + W * i) % EIGHTS;
+            tsrc[i] = A.b + token_row(8 * eight + (lane >> 3)) * A.k_bytes + piece * 16;
+            place[i] = BN * 128 + eight * 1024;
+        }
         f32x4 acc[SN][NT];
 #pragma unroll
         for (int s = 0; s < SN; ++s)
@@ -791,9 +798,8 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
 #pragma unroll
             for (int i = begin; i < end; ++i) {
                 if (i < DW) load_to_lds_16(wbase + off, wsrc[i < DW ? i : 0] + back, at + (wave + W * i) * 1024);
-                else if (i < LOADS) load_to_lds_16(tsrc[i - DW < DT ? i - DW : 0] + off + back, at + BN * 128 + (wave + W * (i - DW)) * 1024,
-                                                   (i - DW + 1) * W > EIGHTS, (wave + W * (i - DW) - EIGHTS) >> 31);
-                else load_to_lds_4(ssrc + kb, at + SCALES + scale_slot * 256, scale_lanes);
+                else if (i < LOADS) load_to_lds_16(tsrc[i - DW < LOADS - DW ? i - DW : 0] + off + back, at + place[i - DW < LOADS - DW ? i - DW : 0]);
+                else load_to_lds_4(ssrc + kb, at + SCALES + wave % SCALE_WAVES * 256, scale_lanes);
             }
         };
 #pragma unroll
