@@ -65,7 +65,8 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
 }
 
 // The groups' bounds, 64 groups a pass, lane by lane; those of the first passes stay in registers, so that their loads are on
-// their way together. Offsets are bounded to [0, n_rows]: bad ones cannot lead out of the buffers.
+// their way together. Offsets are bounded to [0, n_rows]: bad ones cannot lead out of the buffers (n_rows < 2^29, so that the tiles
+// of 64 groups that all span it, 32 rows a tile, are still counted in 31 bits; tiles of fewer rows are for far fewer rows).
 struct Groups {
     static constexpr int KEPT = 4;
     const ProductArgs & A;
@@ -389,6 +390,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
                 issue(i + D);
             }
             drain<D - 1, P>(i, n_steps, compute);
+            landed<0>();                                     // (the next run's loads take the places of this one's last reads)
         }
         __syncthreads();                                     // the rings are free: the waves' sums go there
         f32x4 * parts = reinterpret_cast<f32x4 *>(lds);      // [wave][fragment][lane]
@@ -1043,7 +1045,7 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     require(w.rows > 0 && w.rows < (int64_t{1} << 30) && w.k > 0 && w.k < (int64_t{1} << 23), "rows and k out of range");
     const int64_t k_bytes = w.k * (f8 ? 1 : 2);
     require(k_bytes % 16 == 0, f8 ? "k must be a multiple of 16" : "k must be a multiple of 8");
-    require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 31) && a.n_b >= 0 && a.n_dst >= 0 && a.n_dst < (int64_t{1} << 31) - 2, "row counts out of range");
+    require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 29) && a.n_b >= 0 && a.n_dst >= 0 && a.n_dst < (int64_t{1} << 31) - 2, "row counts out of range");
     require(a.b_div > 0 && a.b_div < (int64_t{1} << 31), "b_div must be positive");
     if (a.n_rows == 0) return;
     require(w.data && b && dst && a.n_b > 0 && (!f8 || (w.scales && b_scales)), "null buffer");
