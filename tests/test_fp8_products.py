@@ -87,6 +87,7 @@ def test_dense_refusals(vb, kw, call, needle):
     ({}, dict(b_div=0), b"b_div"),
     ({}, dict(n_b=0), b"null"),
     ({}, dict(n_b=-1), b"out of range"),
+    ({}, dict(n_rows=1 << 29), b"out of range"),
     ({}, dict(n_dst=-1), b"out of range"),
     ({}, dict(b_scales=None), b"null"),
     ({}, dict(b_rows=P + 2), b"aligned"),
