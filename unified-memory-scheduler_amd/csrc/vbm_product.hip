@@ -1006,8 +1006,8 @@ void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
 //   One wave a row tile from 4096 row tiles on (two for each wave that the card holds); the depth shared among four
 //   waves below that.
 // - 11 to 40 rows: 128 x 64 (128 experts of 1536 x 2048: 16 rows 80, 32 rows 86, against 86 and 90 in tiles of 256 x 256; bf16, 32 experts of 2880 x
-//   2880, 16 rows 100 against 106), 64 x 32 where there are too few of those: 333 tokens x 2880 x 2880 13.9 against 15.4, 100 tokens 10.6
-//   against 15.0; but 700 tokens 23.2 against 16.4, 512 x 4096 x 4096 25.0 against 19.0.
+//   2880, 16 rows 100 against 106), 64 x 32 where there are too few of those: 333 tokens x 2880 x 2880 13.4 against 15.4, 100 tokens 9.6
+//   against 15.0; but 700 tokens 22.5 against 16.1, 512 x 4096 x 4096 24.0 against 18.6.
 // - more: 256 x 256, or 256 x 128 where that leaves CUs idle: 2048 x 2880 x 2880 30 against 46, 2048 x 5760 x 2880 57.5 against 47; and 128 x 64 where
 //   that does too: 2048 x 2048 x 2048 18.9 against 22.0, 1500 x 2880 x 2880 34.5 against 28.8. Groups of more than 140 rows take two
 //   256 x 160 tiles rather than one 256 x 256, which leave LDS for a third stage: 256 rows, 2880 x 2880 137 against 153, bf16 5760 x
