@@ -246,17 +246,12 @@ def _plain(s):
 
 
 # ---------------------------------------------------------------------------- this engine's kernels
-_vbmoe = None
-
-
 def _engine():
-    """The package, imported once, as a program does."""
-    global _vbmoe
-    if _vbmoe is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "unified-memory-scheduler_amd"))
-        import vbmoe
-        _vbmoe = vbmoe
-    return _vbmoe
+    path = str(Path(__file__).resolve().parent.parent / "unified-memory-scheduler_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import vbmoe
+    return vbmoe
 
 
 def _kernels(s):
