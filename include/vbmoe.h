@@ -316,9 +316,10 @@ typedef struct vbm_weights {
 
 /* dst[t][n] = w[n] . b[t] (+ bias[n]) of one FP8 matrix with tokens quantized by vbm_quantize_fp8: b codes
  * [n_tokens][k] (16-byte aligned), b_scales [n_tokens][ceil(k / 128)], dst [n_tokens][rows] of dst_type (F32, F16 or
- * BF16); n_tokens < 2^29. F32 outputs are fp32 sums of exact products. F16 and BF16 outputs are rounded once from fp32 sums in which every
- * eight neighbouring products are added by the FP8 matrix instruction, cut off 13 bits below the largest of them (1e-5 to 6e-5 of
- * the result on random data, a tenth of an F16 rounding's error or less). n_tokens = 0 does nothing. k < 2^23. */
+ * BF16); n_tokens < 2^29. Outputs are rounded once, from fp32 sums of exact products; but the products of BF16 outputs of more
+ * than 10 tokens are added by the FP8 matrix instruction, which cuts every eight neighbouring ones off 13 bits below the leading bit
+ * of the largest: at most 7 * 2^-13 of that one, and on random data 1.4e-5 to 6e-5 of the outputs' root mean square (their rounding to
+ * BF16 is 1.7e-3 of it). Where such a sum cancels, F32 and F16 outputs keep what is left. n_tokens = 0 does nothing. k < 2^23. */
 vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type,
                            void * dst, void * stream);
 
@@ -327,7 +328,7 @@ vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * 
  *   dst[dst_rows ? dst_rows[i] : i] = w[g] . b[b_rows ? b_rows[i] / b_div : i] (+ bias[g])
  * offsets [n_groups + 1] as vbm_group_by_expert writes them, n_rows >= offsets[n_groups] the most rows there
  * can be (its n_ids * n_tokens); neither is read on the host. b is [n_b][k] in the weights' type (F8: codes with
- * b_scales [n_b][ceil(k / 128)]), dst [n_dst][rows] of dst_type; sums as in vbm_mul_mat_fp8. A b row outside [0, n_b) makes its outputs NaN; a dst
+ * b_scales [n_b][ceil(k / 128)]), dst [n_dst][rows] of dst_type; sums as in vbm_mul_mat_fp8 (its tokens: n_rows / n_groups). A b row outside [0, n_b) makes its outputs NaN; a dst
  * row outside [0, n_dst) is not written, nor are dst rows that no group lists. dst_rows must not list a
  * row twice. n_rows < 2^29; n_rows = 0 does nothing. */
 vbm_status vbm_grouped_mul_mat(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_b,

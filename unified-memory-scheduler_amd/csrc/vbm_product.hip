@@ -28,9 +28,13 @@ typedef __bf16 bf16x8_p __attribute__((ext_vector_type(8)));
 // How a step's 128 bytes a row are multiplied.
 //   kF8Wide: the e4m3 codes widened to fp16 (exact) and multiplied as such: exact products, fp32 sums.
 //   kF8: by the FP8 matrix instruction, at twice that rate. It adds eight neighbouring products at a time, aligned to the largest of
-//        them and cut off 13 bits below its leading one (found by probing it with two products of different size); between such
-//        eights it sums in fp32. That is at most 7 * 2^-13 of the largest of eight, and 1.4e-5 to 6e-5 of the result on random data: far
-//        below the rounding of a 16-bit output (2^-9 or 2^-12 on average), which is what it is used for, and too much for fp32 ones.
+//        them and cut off 13 bits below its leading one (found by probing it with two products of different size; the other FP8 matrix
+//        instructions do the same); between such eights it sums in fp32. That is at most 7 * 2^-13 of the largest of eight; on random data
+//        1.4e-5 of the outputs' root mean square for normal codes, 6e-5 for codes of widely different size. Only for bf16 outputs, whose own
+//        rounding is 1.7e-3, and only from 11 rows a group on, where it saves time: 4096 x 4096 x 4096 66 us against 129 widened (which
+//        takes a quarter-rate instruction for every two values), 2048 x 2880 x 2880 30 against 47, 2048 tokens top-8 over 128 experts of
+//        1536 x 2048 123 against 156. Up to 10 rows a group both take as long: one token through 8 experts 9.7 and 9.8, 64 tokens top-4 over
+//        32 experts of 5760 x 2880 103 and 104. An fp16 output's rounding, 2e-4, would not cover it.
 //   kF16, kBF16: as they are.
 enum Kind { kF8Wide, kF8, kF16, kBF16 };
 constexpr bool is_f8(int kind) { return kind == kF8Wide || kind == kF8; }
@@ -1017,13 +1021,14 @@ void launch_product(const ProductArgs & a, hipStream_t stream) {
     if (a.n_rows == 0) return;
     const int64_t groups = std::min<int64_t>(a.n_groups, a.n_rows), mean = a.n_rows / groups;
     if (mean <= 10) {
+        constexpr int FEW = KIND == kF8 ? kF8Wide : KIND;
         const bool wide = groups * ((a.rows + 15) / 16) >= 4096;
         if (mean <= 4) {
-            if (wide && (launch_stream_rows<KIND, 1, 4, 4>(a, groups, stream) || launch_stream_rows<KIND, 1, 8, 4>(a, groups, stream))) return;
-            return launch_few_rows<KIND, 1, 4>(a, stream);
+            if (wide && (launch_stream_rows<FEW, 1, 4, 4>(a, groups, stream) || launch_stream_rows<FEW, 1, 8, 4>(a, groups, stream))) return;
+            return launch_few_rows<FEW, 1, 4>(a, stream);
         }
-        if (wide && (launch_stream_rows<KIND, 2, 4, 3>(a, groups, stream) || launch_stream_rows<KIND, 2, 8, 4>(a, groups, stream))) return;
-        return launch_few_rows<KIND, 2, 3>(a, stream);
+        if (wide && (launch_stream_rows<FEW, 2, 4, 3>(a, groups, stream) || launch_stream_rows<FEW, 2, 8, 4>(a, groups, stream))) return;
+        return launch_few_rows<FEW, 2, 3>(a, stream);
     }
     auto tiles = [&](int64_t bn, int64_t bt) { return (a.rows + bn - 1) / bn * groups * ((mean + bt - 1) / bt); };
     if (mean > 40) {
@@ -1067,7 +1072,7 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     a.rows = static_cast<int>(w.rows);
     a.k_bytes = static_cast<int>(k_bytes);
     a.kb = static_cast<int>((k_bytes + 127) / 128);
-    if (f8 && dst_type != VBM_TYPE_F32) launch_product<kF8>(a, stream);
+    if (f8 && dst_type == VBM_TYPE_BF16) launch_product<kF8>(a, stream);
     else if (f8) launch_product<kF8Wide>(a, stream);
     else if (w.type == VBM_TYPE_F16) launch_product<kF16>(a, stream);
     else launch_product<kBF16>(a, stream);
