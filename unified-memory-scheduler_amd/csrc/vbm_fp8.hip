@@ -98,8 +98,11 @@ __device__ __forceinline__ void store_block(const float v[8], bool live, uint8_t
     if ((threadIdx.x & 15) == 0) *scale = finite ? a / 448.0f : __builtin_nanf("");
 }
 
-// exp(x) for x <= 88 to about an ulp: 2^(x log2 e) by the hardware's 2^y, corrected by what the product's rounding and log2 e's
+// exp(x) for x in [-104, kLastExp] to about an ulp: 2^(x log2 e) by the hardware's 2^y, corrected by what the product's rounding and log2 e's
 // own lost. (expf_rn of the exact order, which rounds from double, would bound these kernels by its arithmetic.)
+// kLastExp: the largest fp32 x whose e^x is one too, 88.7228317 (below ln(2^128 - 2^103) = 88.7228391, and the next one above); x log2 e
+// is then at most 127.99999, and 2^y in range.
+constexpr float kLastExp = 0x1.62e42ep+6f;
 __device__ __forceinline__ float exp_ulp(float x) {
     const float log2e = 1.44269502e+00f, log2e_rest = 1.92596299e-08f, ln2 = 6.93147181e-01f;
     const float hi = x * log2e;
@@ -107,19 +110,21 @@ __device__ __forceinline__ float exp_ulp(float x) {
     const float e = __builtin_amdgcn_exp2f(hi);
     return __builtin_fmaf(e, lo * ln2, e);
 }
-// a / b for b in [1, 2^126]: reciprocal and one Newton step on the quotient.
-__device__ __forceinline__ float quotient(float a, float b) {
-    const float r = __builtin_amdgcn_rcpf(b), q = a * r;
-    return __builtin_fmaf(__builtin_fmaf(-q, b, a), r, q);
+// a / (1 + e^x): reciprocal and one Newton step on the quotient, of a quarter of both, so that the reciprocal of the largest
+// e^x is a normal number. Past the fp32 range of e^x it is a zero, as a division by infinity (NaN for an infinite a).
+__device__ __forceinline__ float over_one_plus_exp(float a, float x) {
+    const float d = __builtin_fmaf(exp_ulp(x < -104.0f ? -104.0f : x), 0.25f, 0.25f), n = 0.25f * a;
+    const float r = __builtin_amdgcn_rcpf(d), q = n * r;
+    return x > kLastExp ? 0.0f * a : __builtin_fmaf(__builtin_fmaf(-q, d, n), r, q);
 }
-// The formulas of glu(). The exponent stops at 87, where 1 / (1 + e^x) is still a normal number.
+// The formulas of glu().
 __device__ __forceinline__ float glu_value(int activation, float g0, float u0, float alpha, float limit) {
     if (activation == VBM_ACT_SWIGLU_OAI) {
         const float g = limit < g0 ? limit : g0;
         const float u = u0 < -limit ? -limit : (limit < u0 ? limit : u0);
-        return quotient(g, 1.0f + exp_ulp(fminf(alpha * -g, 87.0f))) * (u + 1.0f);
+        return over_one_plus_exp(g, alpha * -g) * (u + 1.0f);
     }
-    return quotient(g0, 1.0f + exp_ulp(fminf(-g0, 87.0f))) * u0;
+    return over_one_plus_exp(g0, -g0) * u0;
 }
 
 struct Fp8Args {
