@@ -286,6 +286,9 @@ vbm_status vbm_weighted_combine(const float * y, const float * weights, int64_t 
  *   vbm_grouped_mul_mat     down: dst_rows = rows -> y [n_tokens][top_k][H] (F32)
  *   vbm_weighted_combine    y, weights -> out [n_tokens][H]
  *
+ * The down product does not write the rows of y whose ids are -1 (the grouping skips them), and the combine reads all of y: where
+ * there can be such ids, vbm_memset y to 0 before it (their weights should be 0 too).
+ *
  * None of them allocates, needs a workspace or waits: all can be captured in a HIP graph, and calls on
  * different streams do not share anything. Buffers belong to the current device. Results do not depend on
  * what else runs, and a call repeated on the same inputs gives the same bits.
@@ -855,7 +858,7 @@ vbm_status vbm_graph_compute(const vbm_node * const * nodes, int64_t n_nodes, co
 /* ----------------------------------------------------------------------------------------------
  * HIP graph capture of stream-ordered work (per-token layer chains replay without host launch
  * overhead). Only entry points that do not allocate (the layer forward with a caller workspace,
- * the router, combine, quantize and device copies) may be captured.
+ * the router, combine, quantize, the FP8 and grouped products, device copies and vbm_memset) may be captured.
  * -------------------------------------------------------------------------------------------- */
 vbm_status vbm_graph_begin_capture(void * stream);
 vbm_status vbm_graph_end_capture(void * stream, void ** graph_exec);

@@ -11,6 +11,17 @@
 namespace vbm {
 namespace {
 thread_local std::string g_last_error;
+
+// Four equal bytes over `bytes` bytes from dst on, 16 at a time where they are aligned; the first threads write the ends.
+__global__ void fill_kernel(uint8_t * __restrict__ dst, uint32_t four, size_t bytes) {
+    const size_t to_aligned = (16 - reinterpret_cast<uintptr_t>(dst) % 16) % 16, head = to_aligned < bytes ? to_aligned : bytes;
+    const size_t pieces = (bytes - head) / 16, end = head + 16 * pieces;
+    const size_t first = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x;
+    for (size_t i = first; i < pieces; i += static_cast<size_t>(gridDim.x) * blockDim.x)
+        reinterpret_cast<uint4 *>(dst + head)[i] = uint4{four, four, four, four};
+    if (first < head) dst[first] = static_cast<uint8_t>(four);
+    if (first < bytes - end) dst[end + first] = static_cast<uint8_t>(four);
+}
 }
 void set_last_error(const std::string & message) { g_last_error = message; }
 void clear_last_error() { g_last_error.clear(); }
@@ -84,7 +95,18 @@ vbm_status vbm_memcpy_d2d(void * dst, const void * src, size_t bytes, void * str
 }
 vbm_status vbm_memset(void * dst, int value, size_t bytes, void * stream) {
     return guarded([&] {
-        if (bytes) check_hip(hipMemsetAsync(dst, value, bytes, as_stream(stream)), "hipMemsetAsync");
+        if (!bytes) return;
+        // (a memset node of a HIP graph has written wrong values on replays after the first: a captured call is a kernel)
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (stream) check_hip(hipStreamIsCapturing(as_stream(stream), &capture), "hipStreamIsCapturing");
+        if (capture == hipStreamCaptureStatusNone) {
+            check_hip(hipMemsetAsync(dst, value, bytes, as_stream(stream)), "hipMemsetAsync");
+            return;
+        }
+        const size_t groups = std::min<size_t>((bytes / 16 + 255) / 256 + 1, 1u << 16);
+        hipLaunchKernelGGL(fill_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, as_stream(stream), static_cast<uint8_t *>(dst),
+                           static_cast<uint32_t>(value & 0xFF) * 0x01010101u, bytes);
+        check_hip(hipGetLastError(), "fill launch");
     });
 }
 vbm_status vbm_stream_create(void ** stream) {
