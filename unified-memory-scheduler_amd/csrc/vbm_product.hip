@@ -69,8 +69,9 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
 }
 
 // The groups' bounds, 64 groups a pass, lane by lane; those of the first passes stay in registers, so that their loads are on
-// their way together. Offsets are bounded to [0, n_rows]: bad ones cannot lead out of the buffers (n_rows < 2^29, so that the tiles
-// of 64 groups that all span it, 32 rows a tile, are still counted in 31 bits; tiles of fewer rows are for far fewer rows).
+// their way together. Offsets are bounded to [0, n_rows]: bad ones cannot lead out of the buffers. (n_rows < 2^29, so that the tiles
+// of a pass of 64 groups that all span it, 32 rows a tile, are counted in 31 bits; tiles of fewer rows are for far fewer rows. A place
+// is looked for pass by pass, and found before the sum of the passes could leave them.)
 struct Groups {
     static constexpr int KEPT = 4;
     const ProductArgs & A;
@@ -663,8 +664,9 @@ struct Work {
 };
 // The calling workgroup's share: a row tile x a token tile of at most `most` 16-token columns of one group. Workgroup i runs on XCD
 // i % 8, so each XCD takes a contiguous run of the list (group by group, row tile by row tile): the token tiles that share a row
-// tile's weights, and the row tiles that share the tokens, then meet in one L2. A group's tiles share its columns evenly.
-__device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int row_tiles, Work & w) {
+// tile's weights, and the row tiles that share the tokens, then meet in one L2. A group's tiles share its columns evenly. `launched`: the
+// most token tiles that rows grouped in order can have; offsets out of order may count more, and have the first ones done.
+__device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int row_tiles, int launched, Work & w) {
     const int n_rows = static_cast<int>(A.n_rows), slot = static_cast<int>(blockIdx.x >> 3);
     auto columns = [&](int lo, int hi) { return hi > lo ? (hi - lo + 15) >> 4 : 0; };
     auto tiles_of = [&](int lo, int hi) { return (columns(lo, hi) + most - 1) / most; };
@@ -682,10 +684,10 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
         const Groups groups(A);
         int part = 0, sum = 0;
         groups.each([&](int, int l, int h) {
-            part += tiles_of(l, h);
+            part = std::min(part + tiles_of(l, h), launched);    // (below 2^24: the sum of 64 lanes is counted in 31 bits)
             return false;
         });
-        if (!mine(__builtin_amdgcn_readlane(wave_inclusive_sum(part), 63))) return false;
+        if (!mine(std::min(__builtin_amdgcn_readlane(wave_inclusive_sum(part), 63), launched))) return false;
         const int index = item / row_tiles;
         groups.each([&](int g0, int l, int h) {
             Place p;
@@ -697,6 +699,7 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
             before = p.before;
             return true;
         });
+        if (!tiles) return false;
     }
     const int local = item - before * row_tiles;
     w.row_tile = local / tiles;
@@ -719,14 +722,14 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 // runs: the same here, 5 % slower for ragged groups. Grouped prefill is bound by the weights' stream and what a workgroup
 // does not overlap with it: one of them fits a CU, and its start (bounds, rows, first stages) and end cost about 8 us of some 40.
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
-__global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles) {
+__global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles, int launched) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
     constexpr int DW = BN / 8 / W;                           // a wave's loads of weights a step: 8 rows each
     static_assert(DW * 8 * W == BN && BT % 32 == 0, "the waves share the loads");
     constexpr int STAGE_BYTES = LDS - BT * 4;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
     Work work;
-    if (!find_work(A, ST * WT, row_tiles, work)) return;
+    if (!find_work(A, ST * WT, row_tiles, launched, work)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int q = lane >> 4, r = lane & 15, wn = wave / WT, wt = wave % WT;
     const int n0 = work.row_tile * BN;
@@ -997,10 +1000,10 @@ bool launch_stream_rows(const ProductArgs & a, int64_t groups, hipStream_t strea
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 void launch_many_rows(const ProductArgs & a, hipStream_t stream) {
     constexpr int BN = 16 * SN * WN, BT = 16 * ST * WT;
-    const int64_t row_tiles = (a.rows + BN - 1) / BN, items = row_tiles * most_token_tiles(a, BT);
+    const int64_t row_tiles = (a.rows + BN - 1) / BN, tiles = most_token_tiles(a, BT), items = row_tiles * tiles;
     require(items < (int64_t{1} << 32) / (WN * WT * 64) - 8, "too many outputs for one launch");
     hipLaunchKernelGGL((many_rows_kernel<KIND, SN, ST, WN, WT, LDS>), dim3(static_cast<unsigned>((items + 7) / 8 * 8)),
-                       dim3(WN * WT * 64), 0, stream, a, static_cast<int>(row_tiles));
+                       dim3(WN * WT * 64), 0, stream, a, static_cast<int>(row_tiles), static_cast<int>(tiles));
     check_hip(hipGetLastError(), "product launch");
 }
 
