@@ -24,7 +24,6 @@ namespace {
 constexpr int kFp8Threads = 256;
 constexpr int kBlocksPerGroup = kFp8Threads / 16;
 
-typedef _Float16 half8_q __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4q __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2q __attribute__((ext_vector_type(2)));
 

@@ -271,7 +271,7 @@ __device__ __forceinline__ void drain(int i, int n, const F & compute) {
 }
 
 // ------------------------------------------------------------------------------- few tokens a group
-// A workgroup takes 16 * RS weight rows x up to 8 * MAX8 tokens of one group; its W waves share the depth in runs and add their
+// A workgroup takes 16 weight rows x up to 8 * MAX8 tokens (MAX8: 1 or 2) of one group; its W waves share the depth in runs and add their
 // sums up through LDS, in wave order. The weights' bytes are the work, and they are read once; what counts is that enough of them
 // are on their way. Each wave streams its own through a ring of D steps in LDS, without barriers: a load brings 128
 // bytes of each of eight rows, in neighbouring lanes (loaded straight into a matrix operand's registers, 16 rows in neighbouring lanes,
@@ -280,13 +280,13 @@ __device__ __forceinline__ void drain(int i, int n, const F & compute) {
 // through one matrix of 5760 x 2880: 5.9 us, latency: bounds and rows, the weights, the waves' sums.
 template <int KIND, int MAX8, int D>
 __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_tiles) {
-    constexpr int RS = 1;
-    constexpr int W = 4, NT_MAX = (MAX8 + 1) / 2, RUN = 16;  // RUN: steps whose scales a wave holds
-    constexpr int STEP = (2 * RS + MAX8) * 1024, SCALES = is_f8(KIND) ? RUN * 64 * NT_MAX : 0, WAVE = D * STEP + SCALES;
-    static_assert(W * RS * NT_MAX * 1024 <= W * WAVE, "the ring's memory holds the waves' sums");
+    static_assert(MAX8 <= 2, "one column of sixteen tokens");
+    constexpr int W = 4, RUN = 16;                           // RUN: steps whose scales a wave holds
+    constexpr int STEP = (2 + MAX8) * 1024, SCALES = is_f8(KIND) ? RUN * 64 : 0, WAVE = D * STEP + SCALES;
+    static_assert(1024 <= WAVE, "the ring's memory holds the waves' sums");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[W * WAVE];
     TokenTile t;
-    const int token_tile = static_cast<int>(blockIdx.x) / row_tiles, n0 = (static_cast<int>(blockIdx.x) - token_tile * row_tiles) * (16 * RS);
+    const int token_tile = static_cast<int>(blockIdx.x) / row_tiles, n0 = (static_cast<int>(blockIdx.x) - token_tile * row_tiles) * 16;
     if (!find_token_tile(A, token_tile, 8 * MAX8, t)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int q = lane >> 4, r = lane & 15, live = static_cast<int>(t.last - t.first);
@@ -298,9 +298,9 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
     };
 
     const uint8_t * wbase = A.w + (static_cast<int64_t>(t.group) * A.rows + n0) * A.k_bytes;
-    uint32_t wsrc[2 * RS];
+    uint32_t wsrc[2];
 #pragma unroll
-    for (int i = 0; i < 2 * RS; ++i) {
+    for (int i = 0; i < 2; ++i) {
         const int n = n0 + 8 * i + (lane >> 3);
         wsrc[i] = static_cast<uint32_t>((n < A.rows ? n : A.rows - 1) - n0) * static_cast<uint32_t>(A.k_bytes);
     }
@@ -308,20 +308,14 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
     const int k_begin = A.kb * wave / W, k_end = A.kb * (wave + 1) / W;
 
     auto run = [&](auto t8_c) __attribute__((always_inline)) {
-        constexpr int T8 = decltype(t8_c)::value, NT = (T8 + 1) / 2, P = 2 * RS + T8;   // P: loads a step
+        constexpr int T8 = decltype(t8_c)::value, P = 2 + T8;   // P: loads a step
         const uint8_t * tsrc[T8];
 #pragma unroll
         for (int i = 0; i < T8; ++i) tsrc[i] = A.b + token_row(8 * i + (lane >> 3)) * A.k_bytes;
-        const float * ssrc[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) ssrc[j] = is_f8(KIND) ? A.bs + token_row(16 * j + (lane >> 2)) * A.kb : nullptr;
+        const float * ssrc = is_f8(KIND) ? A.bs + token_row(lane >> 2) * A.kb : nullptr;
         // piece lane % 8 of a row sits at its place xor (row / 2 % 8), as in the kernels below
         const int piece_even = (lane & 7) ^ (lane >> 4), piece_odd = piece_even ^ 4;
-        f32x4 acc[RS][NT];
-#pragma unroll
-        for (int s = 0; s < RS; ++s)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[s][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
 
         for (int k0 = k_begin; k0 < k_end; k0 += RUN) {
             const int n_steps = k_end - k0 < RUN ? k_end - k0 : RUN;
@@ -330,12 +324,10 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
                 scales = lane < n_steps ? wscale[k0 + lane] : 0.0f;
                 asm volatile("" : "+v"(scales));
                 // the tokens' scales, four steps of sixteen tokens a load: [four steps][token][4]
-                for (int c = 0; c < (n_steps + 3) / 4; ++c)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const int k = k0 + 4 * c + (lane & 3);
-                        load_to_lds_4(ssrc[j] + (k < A.kb ? k : A.kb - 1), lds0 + D * STEP + (c * NT_MAX + j) * 256);
-                    }
+                for (int c = 0; c < (n_steps + 3) / 4; ++c) {
+                    const int k = k0 + 4 * c + (lane & 3);
+                    load_to_lds_4(ssrc + (k < A.kb ? k : A.kb - 1), lds0 + D * STEP + c * 256);
+                }
             }
             auto issue = [&](int i) __attribute__((always_inline)) {
                 const int k = k0 + i;
@@ -344,17 +336,15 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
                 // (a piece past the row's end reads the step's first one: zeros take its place in the registers)
                 const int even = k * 128 + piece_even * 16 < A.k_bytes ? piece_even * 16 : 0, odd = k * 128 + piece_odd * 16 < A.k_bytes ? piece_odd * 16 : 0;
 #pragma unroll
-                for (int l = 0; l < 2 * RS; ++l) load_to_lds_16(wbase + off, wsrc[l] + (l & 1 ? odd : even), at + l * 1024);
+                for (int l = 0; l < 2; ++l) load_to_lds_16(wbase + off, wsrc[l] + (l & 1 ? odd : even), at + l * 1024);
 #pragma unroll
-                for (int l = 0; l < T8; ++l) load_to_lds_16(tsrc[l] + off + (l & 1 ? odd : even), at + (2 * RS + l) * 1024);
+                for (int l = 0; l < T8; ++l) load_to_lds_16(tsrc[l] + off + (l & 1 ? odd : even), at + (2 + l) * 1024);
             };
             auto compute = [&](int i) __attribute__((always_inline)) {
                 const uint8_t * stage = mine + (i % D) * STEP;
                 const int left = A.k_bytes - (k0 + i) * 128 - 32 * q;   // bytes of the row from this lane's pieces on
-                auto operand = [&](int row) __attribute__((always_inline)) {
-                    // row r of sixteen; of eight tokens rows 8 .. 15 read rows 0 .. 7 (their columns are not used)
-                    const int rr = row >= 2 * RS * 8 && T8 == 1 ? r & 7 : r;
-                    const uint8_t * p = stage + row * 128 + rr * 128;
+                auto operand = [&](const uint8_t * rows, int rr) __attribute__((always_inline)) {
+                    const uint8_t * p = rows + rr * 128;
                     Piece v{*reinterpret_cast<const u32x4p *>(p + ((2 * q) ^ (rr >> 1)) * 16), *reinterpret_cast<const u32x4p *>(p + ((2 * q + 1) ^ (rr >> 1)) * 16)};
                     if (left < 32) {
                         if (left <= 16) v.hi = u32x4p{0, 0, 0, 0};
@@ -364,26 +354,16 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
                     o.take(v);
                     return o;
                 };
-                Operand<KIND> a[RS];
+                // (of eight tokens rows 8 .. 15 read rows 0 .. 7: their columns are not used)
+                const Operand<KIND> a = operand(stage, r), b = operand(stage + 2048, T8 == 1 ? r & 7 : r);
+                if constexpr (is_f8(KIND)) {
+                    const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scales), i));
+                    const float f = sw * *reinterpret_cast<const float *>(mine + D * STEP + (i >> 2) * 256 + r * 16 + (i & 3) * 4);
+                    const f32x4 p = product<KIND>(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-                for (int s = 0; s < RS; ++s) a[s] = operand(16 * s);
-                float sw = 0.0f;
-                if constexpr (is_f8(KIND)) sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scales), i));
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const Operand<KIND> b = operand(16 * (RS + j));
-                    if constexpr (is_f8(KIND)) {
-                        const float f = sw * *reinterpret_cast<const float *>(mine + D * STEP + ((i >> 2) * NT_MAX + j) * 256 + r * 16 + (i & 3) * 4);
-#pragma unroll
-                        for (int s = 0; s < RS; ++s) {
-                            const f32x4 p = product<KIND>(a[s], b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[s][j][e] = __builtin_fmaf(p[e], f, acc[s][j][e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < RS; ++s) acc[s][j] = product<KIND>(a[s], b, acc[s][j]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], f, acc[e]);
+                } else {
+                    acc = product<KIND>(a, b, acc);
                 }
             };
             for (int i = 0; i < D && i < n_steps; ++i) issue(i);
@@ -398,39 +378,28 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
             landed<0>();                                     // (the next run's loads take the places of this one's last reads)
         }
         __syncthreads();                                     // the rings are free: the waves' sums go there
-        f32x4 * parts = reinterpret_cast<f32x4 *>(lds);      // [wave][fragment][lane]
-#pragma unroll
-        for (int s = 0; s < RS; ++s)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) parts[(wave * RS * NT + s * NT + j) * 64 + lane] = acc[s][j];
+        f32x4 * parts = reinterpret_cast<f32x4 *>(lds);      // [wave][lane]
+        parts[wave * 64 + lane] = acc;
         __syncthreads();
+        if (wave) return;
+        f32x4 v = parts[lane];
 #pragma unroll
-        for (int f = 0; f < RS * NT; ++f) {
-            if (f % W != wave) continue;
-            const int s = f / NT, j = f % NT;
-            f32x4 v = parts[f * 64 + lane];
+        for (int w = 1; w < W; ++w) v += parts[w * 64 + lane];
+        const int n = n0 + 4 * q;
+        const int64_t i = t.first + r;
+        if (i >= t.last || n >= A.rows) return;
+        const int64_t row = target_row(A, i);
+        if (row < 0) return;
+        if (A.bias) {
 #pragma unroll
-            for (int w = 1; w < W; ++w) v += parts[(w * RS * NT + f) * 64 + lane];
-            const int n = n0 + 16 * s + 4 * q;
-            const int64_t i = t.first + 16 * j + r;
-            if (i >= t.last || n >= A.rows) continue;
-            const int64_t row = target_row(A, i);
-            if (row < 0) continue;
-            if (A.bias) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(t.group) * A.rows + n + e];
-            }
-            const float nan = __builtin_nanf("");
-            store4(A, row, n, source_row(A, i) < 0 ? f32x4{nan, nan, nan, nan} : v);
+            for (int e = 0; e < 4; ++e)
+                if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(t.group) * A.rows + n + e];
         }
+        const float nan = __builtin_nanf("");
+        store4(A, row, n, source_row(A, i) < 0 ? f32x4{nan, nan, nan, nan} : v);
     };
-    const int eights = (live + 7) >> 3;
-    if constexpr (MAX8 >= 4) {
-        if (eights > 2) return run(std::integral_constant<int, 4>{});
-    }
-    if constexpr (MAX8 >= 2) {
-        if (eights > 1) return run(std::integral_constant<int, 2>{});
+    if constexpr (MAX8 == 2) {
+        if (live > 8) return run(std::integral_constant<int, 2>{});
     }
     run(std::integral_constant<int, 1>{});
 }
@@ -442,13 +411,14 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
 // 2880: 82 us, 5.7 TB/s. Bound by memory.
 template <int KIND, int MAX8, int W, int D>
 struct StreamLayout {
-    static constexpr int NT = (MAX8 + 1) / 2, MAX_TILES = 4;
+    static_assert(MAX8 <= 2, "one column of sixteen tokens");
+    static constexpr int MAX_TILES = 4;
     static constexpr int TOTAL = W * 20 * 1024;              // two workgroups of 4 waves, or one of 8, a CU
     static constexpr int RING = W * D * 2048, ROWS = W * MAX_TILES * 16, BLOCKS = ROWS / 128 + 2;
     static constexpr int BIAS = RING, BLOCK_SCALES = BIAS + ROWS * 4, TOKENS = BLOCK_SCALES + (is_f8(KIND) ? BLOCKS * 256 : 0);
-    static constexpr int STEP = MAX8 * 1024 + (is_f8(KIND) ? NT * 64 : 0);   // a step of the tokens and their scales
+    static constexpr int STEP = MAX8 * 1024 + (is_f8(KIND) ? 64 : 0);   // a step of the tokens and their scales
     // steps that fit (scales come in fours; the weights' scales of 64 steps are kept)
-    static constexpr int FIT = (TOTAL - TOKENS - (is_f8(KIND) ? 4 * NT * 64 : 0)) / STEP;
+    static constexpr int FIT = (TOTAL - TOKENS - (is_f8(KIND) ? 4 * 64 : 0)) / STEP;
     static constexpr int MAX_KB = is_f8(KIND) && FIT > 64 ? 64 : FIT;
 };
 template <int KIND, int MAX8, int W, int D>
@@ -514,15 +484,13 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
             else *reinterpret_cast<u32x4p *>(lds + at + lane * 16) = u32x4p{0, 0, 0, 0};
         }
     }
-    const int scales_at = L::TOKENS + eights * A.kb * 1024, fours = (eights + 1) >> 1;   // fours: 16-token columns
+    const int scales_at = L::TOKENS + eights * A.kb * 1024;
     const int blocks = (A.rows + 127) >> 7;
     if constexpr (is_f8(KIND)) {
-        for (int j = 0; j < fours; ++j) {
-            const float * src = A.bs + token_row(16 * j + (lane >> 2)) * A.kb;
-            for (int c = wave; 4 * c < A.kb; c += W) {
-                const int kb = 4 * c + (lane & 3);
-                load_to_lds_4(src + (kb < A.kb ? kb : A.kb - 1), lds0 + scales_at + (c * fours + j) * 256);
-            }
+        const float * src = A.bs + token_row(lane >> 2) * A.kb;
+        for (int c = wave; 4 * c < A.kb; c += W) {
+            const int kb = 4 * c + (lane & 3);
+            load_to_lds_4(src + (kb < A.kb ? kb : A.kb - 1), lds0 + scales_at + c * 256);
         }
         for (int i = wave; i < L::BLOCKS; i += W) {
             const int block = (n0 >> 7) + i < blocks ? (n0 >> 7) + i : blocks - 1;
@@ -532,27 +500,19 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
     float * bias = reinterpret_cast<float *>(lds + L::BIAS);
     for (int i = threadIdx.x; i < W * 16 * tiles; i += W * 64)
         bias[i] = A.bias && n0 + i < A.rows ? A.bias[static_cast<int64_t>(t.group) * A.rows + n0 + i] : 0.0f;
-    int64_t to[L::NT];                                       // dst rows of token 16 j + r; -1: none
-    bool bad[L::NT];
-#pragma unroll
-    for (int j = 0; j < L::NT; ++j) {
-        const int64_t i = t.first + 16 * j + r;
-        to[j] = i < t.last ? target_row(A, i) : -1;
-        bad[j] = to[j] >= 0 && source_row(A, i) < 0;
-    }
+    const int64_t mine = t.first + r, to = mine < t.last ? target_row(A, mine) : -1;   // the dst row of token r; -1: none
+    const bool bad = to >= 0 && source_row(A, mine) < 0;
     landed<0>();
     __syncthreads();
 
     auto run = [&](auto t8_c) __attribute__((always_inline)) {
-        constexpr int T8 = decltype(t8_c)::value, NT = (T8 + 1) / 2;
+        constexpr int T8 = decltype(t8_c)::value;
         const uint8_t * ring = lds + wave * (D * 2048);
         int slot = 0;
         for (int i = 0; i < my_tiles; ++i) {
             const int n = (first_tile + W * i) * 16;
             const float * wscale = reinterpret_cast<const float *>(lds + L::BLOCK_SCALES + ((n >> 7) - (n0 >> 7)) * 256);
-            f32x4 acc[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
             for (int kb = 0; kb < A.kb; ++kb) {
                 landed<(D - 1) * 2>();
                 const int left = A.k_bytes - kb * 128 - 32 * q;   // bytes of the row from this lane's pieces on
@@ -568,21 +528,16 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
                     return o;
                 };
                 const Operand<KIND> a = operand(ring + slot * 2048 + (r >> 3) * 1024, r, true);
-                float sw = 0.0f;
-                if constexpr (is_f8(KIND)) sw = wscale[kb];
+                // (of eight tokens rows 8 .. 15 read rows 0 .. 7: their columns are not used)
+                const int rr = T8 == 1 ? r & 7 : r;
+                const Operand<KIND> b = operand(lds + L::TOKENS + ((rr >> 3) * A.kb + kb) * 1024, rr, false);
+                if constexpr (is_f8(KIND)) {
+                    const f32x4 p = product<KIND>(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    const float f = wscale[kb] * *reinterpret_cast<const float *>(lds + scales_at + (kb >> 2) * 256 + r * 16 + (kb & 3) * 4);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    // (of eight tokens rows 8 .. 15 read rows 0 .. 7: their columns are not used)
-                    const int rr = 2 * j + 1 == T8 ? r & 7 : r;
-                    const Operand<KIND> b = operand(lds + L::TOKENS + ((2 * j + (rr >> 3)) * A.kb + kb) * 1024, rr, false);
-                    if constexpr (is_f8(KIND)) {
-                        const f32x4 p = product<KIND>(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                        const float f = sw * *reinterpret_cast<const float *>(lds + scales_at + ((kb >> 2) * fours + j) * 256 + r * 16 + (kb & 3) * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[j][e] = __builtin_fmaf(p[e], f, acc[j][e]);
-                    } else {
-                        acc[j] = product<KIND>(a, b, acc[j]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], f, acc[e]);
+                } else {
+                    acc = product<KIND>(a, b, acc);
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
                 issue();
@@ -590,17 +545,11 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
             }
             const f32x4 extra = *reinterpret_cast<const f32x4 *>(bias + (n - n0) + 4 * q);
             const float nan = __builtin_nanf("");
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                if (to[j] >= 0 && n + 4 * q < A.rows) store4(A, to[j], n + 4 * q, bad[j] ? f32x4{nan, nan, nan, nan} : acc[j] + extra);
+            if (to >= 0 && n + 4 * q < A.rows) store4(A, to, n + 4 * q, bad ? f32x4{nan, nan, nan, nan} : acc + extra);
         }
         landed<0>();                                         // no load may land after the workgroup has ended
     };
-    if constexpr (MAX8 >= 4) {
-        if (eights > 3) return run(std::integral_constant<int, 4>{});
-        if (eights > 2) return run(std::integral_constant<int, 3>{});
-    }
-    if constexpr (MAX8 >= 2) {
+    if constexpr (MAX8 == 2) {
         if (eights > 1) return run(std::integral_constant<int, 2>{});
     }
     run(std::integral_constant<int, 1>{});
