@@ -295,12 +295,12 @@ vbm_status vbm_weighted_combine(const float * y, const float * weights, int64_t 
  * -------------------------------------------------------------------------------------------- */
 /* Rows of x (F32, F16 or BF16; row stride x_stride elements) -> e4m3 codes [n_rows][k] (16-byte aligned) and
  * fp32 scales [n_rows][ceil(k / 128)]; k a multiple of 16. For a run of 128 values (the last one of a row
- * may be shorter) with a = max(max |x|, 2^-116): scale = a / 448, code = e4m3(448 x / a), the quotient
- * correctly rounded in fp32 and then to the nearest e4m3 value, ties to even. A run that holds a NaN or an
+ * may be shorter) with a = max(max |x|, 2^-116): scale = a / 448, code = e4m3(448 x / a): 448 x rounded to fp32 (exact for F16 and BF16),
+ * its quotient by a correctly rounded to fp32, and that to the nearest e4m3 value, ties to even. A run that holds a NaN or an
  * infinity gets the scale NaN and zero codes. n_rows = 0 does nothing. */
 vbm_status vbm_quantize_fp8(int x_type, const void * x, int64_t n_rows, int64_t k, int64_t x_stride, void * codes,
                             float * scales, void * stream);
-/* act(gate, up) of vbm_glu (activation, alpha, limit as there) in fp32, quantized as by vbm_quantize_fp8:
+/* act(gate, up) of vbm_glu (activation, alpha, limit as there) in fp32, each operation to about an ulp, quantized as by vbm_quantize_fp8:
  * gate and up rows of `width` values of x_type with their own strides (the halves of a fused gate_up row:
  * up = gate + width, both strides 2 * width). */
 vbm_status vbm_glu_quantize_fp8(int activation, int x_type, const void * gate, const void * up, int64_t n_rows,
@@ -322,7 +322,7 @@ typedef struct vbm_weights {
  * BF16); n_tokens < 2^29. Outputs are rounded once, from fp32 sums of exact products; but the products of BF16 outputs of more
  * than 10 tokens are added by the FP8 matrix instruction, which cuts every eight neighbouring ones off 13 bits below the leading bit
  * of the largest: at most 7 * 2^-13 of that one, and on random data 1.4e-5 to 6e-5 of the outputs' root mean square (their rounding to
- * BF16 is 1.7e-3 of it). Where such a sum cancels, F32 and F16 outputs keep what is left. n_tokens = 0 does nothing. k < 2^23. */
+ * BF16 is 1.7e-3 of it). Where such a sum cancels, F32 and F16 outputs keep what is left. The product of two scales is rounded to fp32. n_tokens = 0 does nothing. k < 2^23. */
 vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type,
                            void * dst, void * stream);
 
@@ -330,7 +330,7 @@ vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * 
  * [offsets[g], offsets[g + 1]),
  *   dst[dst_rows ? dst_rows[i] : i] = w[g] . b[b_rows ? b_rows[i] / b_div : i] (+ bias[g])
  * offsets [n_groups + 1] as vbm_group_by_expert writes them, n_rows >= offsets[n_groups] the most rows there
- * can be (its n_ids * n_tokens); neither is read on the host. b is [n_b][k] in the weights' type (F8: codes with
+ * can be (its n_ids * n_tokens), by whose mean a group the kernel is chosen; neither is read on the host. b is [n_b][k] (n_b > 0) in the weights' type (F8: codes with
  * b_scales [n_b][ceil(k / 128)]), dst [n_dst][rows] of dst_type; sums as in vbm_mul_mat_fp8 (its tokens: n_rows / n_groups). A b row outside [0, n_b) makes its outputs NaN; a dst
  * row outside [0, n_dst) is not written, nor are dst rows that no group lists. dst_rows must not list a
  * row twice. n_rows < 2^29; n_rows = 0 does nothing. */

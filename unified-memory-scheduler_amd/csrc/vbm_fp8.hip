@@ -4,7 +4,7 @@
 // A run of 128 values (the last of a row may be shorter) with a = max(max |x|, 2^-116):
 //   scale = a / 448,  code = e4m3(448 x / a), rounded to nearest even.
 // 448 is the largest e4m3 value, so nothing saturates. 16-bit inputs meet exact ties of the e4m3 grid often, so the
-// quotient is the correctly rounded one: with r = 1 / a correctly rounded, q = x r and one Newton step
+// quotient of 448 x (rounded to fp32, which is exact for them) is the correctly rounded one: with r = 1 / a correctly rounded, q = x r and one Newton step
 // q + (x - q a) r with fused multiply-adds is the rounded x / a (Markstein, "Computation of elementary functions on the
 // IBM RISC System/6000 processor", 1990), two instructions per value instead of a division. a / 512 and 0.875 x stand for a
 // and 448 x, so that neither overflows. The floor under a keeps 1 / a finite; blocks of zeros get its scale. A block with a NaN
@@ -12,7 +12,7 @@
 //
 // Bound by bandwidth (one read of the inputs, one write of a quarter to half of them). Sixteen lanes share a block, eight values
 // each: 16- or 2 x 16-byte loads, an 8-byte store of codes, and the maximum over 16 lanes by four DPP moves. 8192 x 4096 bf16 19 to
-// 21 us (5.0 TB/s), GLU of 8192 x 2880 fp32 pairs 33 to 40 us (5.3 TB/s, where a large copy reaches 5.1); one row 2 us, a launch.
+// 21 us (5.0 TB/s), GLU of 8192 x 2880 fp32 pairs 41 us (5.2 TB/s, where a large copy reaches 5.1); one row 2 us, a launch.
 #include <type_traits>
 
 #include "vbm_device.hpp"

@@ -263,8 +263,9 @@ __device__ __forceinline__ void drain(int i, int n, const F & compute) {
 // are on their way. Each wave streams its own through a ring of D steps in LDS, without barriers: a load brings 128
 // bytes of each of eight rows, in neighbouring lanes (loaded straight into a matrix operand's registers, 16 rows in neighbouring lanes,
 // a kilobyte occupies the address unit for 64 cycles instead of 18, which alone limits a CU to 16 bytes a cycle).
-// One token through eight FP8 experts of 1536 x 2048: 6.4 us, of which the 25 MB take 5 at the rate of a large copy; one token
-// through one matrix of 5760 x 2880: 5.9 us, latency: bounds and rows, the weights, the waves' sums.
+// One token through eight FP8 experts of 1536 x 2048: 9.2 us (7.1 from the caches), of which the 25 MB take 5 at the rate of a large
+// copy; one token through one matrix of 5760 x 2880: 6.3 us, latency: bounds and rows, the weights, the waves' sums. Deep rows of many
+// experts (64 tokens top-4 over 32 experts, FP8 2880 x 7168 118 us, bf16 2880 x 4096 127) are read at 5.6 to 5.9 TB/s.
 template <int KIND, int MAX8, int D>
 __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_tiles) {
     static_assert(MAX8 <= 2, "one column of sixteen tokens");
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
 // The same where there are rows enough to keep the card busy with one wave a row tile: the tokens, of all of the depth, are staged in LDS
 // once and shared by the workgroup's W waves; then each wave streams `tiles` row tiles of 16 rows, one after the other through
 // a ring of D steps, with no barrier and no sums to join. 64 tokens top-4 over 32 FP8 experts of 5760 x 2880, fp32 outputs: 106 us,
-// 5.05 TB/s (a large copy reaches 5.1); with the depth shared among the waves 134..163. 16 tokens top-4 over 32 bf16 experts of 2880 x
+// 5.05 TB/s (a large copy reaches 5.1); with the depth shared among the waves (the kernel above) 135. 16 tokens top-4 over 32 bf16 experts of 2880 x
 // 2880: 82 us, 5.7 TB/s. Bound by memory.
 template <int KIND, int MAX8, int W, int D>
 __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int row_units, int tiles) {
@@ -638,7 +639,7 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 // wait and one barrier a step. Piece p (16 bytes) of row r lies at place p ^ (r / 2 % 8) of the row's 128 bytes: sixteen rows'
 // reads of one piece then cover all banks (unswizzled they took twice as long).
 //
-// FP8 4096 x 4096 x 4096 with 16-bit outputs: 65 to 67 us, 2.1 PFLOP/s, where a library's product without block scales reaches 2.7.
+// FP8 4096 x 4096 x 4096 with bf16 outputs: 65 to 67 us, 2.1 PFLOP/s, where a library's product without block scales reaches 2.7.
 // Per step of 256 x 256 (1.75 us): the matrix instructions alone 1.0, with the fp32 sums of the scaled blocks 1.25 (an FMA per output and
 // block, half of a matrix instruction's time), the LDS reads under them; the rest is the loads' issue: a wave stands still until
 // the address unit has taken its kilobyte (18 cycles each, 64 of them a step), and the waves of a workgroup ask for it together.

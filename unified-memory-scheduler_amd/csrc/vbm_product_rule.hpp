@@ -14,8 +14,8 @@ namespace vbm {
 //        1.4e-5 of the outputs' root mean square for normal codes, 6e-5 for codes of widely different size. Only for bf16 outputs, whose own
 //        rounding is 1.7e-3, and only from 11 rows a group on, where it saves time: 4096 x 4096 x 4096 66 us against 129 widened (which
 //        takes a quarter-rate instruction for every two values), 2048 x 2880 x 2880 30 against 47, 2048 tokens top-8 over 128 experts of
-//        1536 x 2048 123 against 156. Up to 10 rows a group both take as long: one token through 8 experts 9.7 and 9.8, 64 tokens top-4 over
-//        32 experts of 5760 x 2880 103 and 104. An fp16 output's rounding, 2e-4, would not cover it.
+//        1536 x 2048 123 against 156. Up to 10 rows a group both take as long: one token through 8 experts 9.2 (7.1 against 6.6 with the
+//        weights in the caches), 64 tokens top-4 over 32 experts of 5760 x 2880 103 and 104. An fp16 output's rounding, 2e-4, would not cover it.
 //   kF16, kBF16: as they are.
 enum Kind { kF8Wide, kF8, kF16, kBF16 };
 constexpr bool is_f8(int kind) { return kind == kF8Wide || kind == kF8; }
@@ -34,7 +34,9 @@ struct StreamLayout {
     static constexpr int MAX_KB = is_f8(KIND) && FIT > 64 ? 64 : FIT;
 };
 
-// Which kernel, by the rows a group has on average and the tiles that a launch then has for 256 CUs (us, FP8 unless said otherwise):
+// Which kernel, by the rows a group has on average (of n_rows, the most there can be: how they lie is not known on the host; all 512 in one
+// of 128 experts of 1536 x 2048 take 32 us, evenly spread 91) and the tiles that a launch then has for 256 CUs (us, FP8 unless said
+// otherwise; bf16 outputs from 11 rows on):
 // - up to 10 rows: the streaming kernels. 32 experts of 5760 x 2880, 8 rows 107, 10 rows 108, 12 rows 114 and 16 rows 133, against 109, 111,
 //   112 and 115 in tiles of 128 x 64. Tokens by eights up to 4 rows: 16-bit experts of 2880 x 2880, 2 rows 82 against 85.
 //   One wave a row tile from 4096 row tiles on (two for each wave that the card holds); the depth shared among four
