@@ -44,6 +44,7 @@ enum {
     VBM_TYPE_F32 = 0,
     VBM_TYPE_F16 = 1,
     VBM_TYPE_Q8_0 = 8,
+    VBM_TYPE_I8 = 24,
     VBM_TYPE_I32 = 26,
     VBM_TYPE_BF16 = 30,
     VBM_TYPE_MXFP4 = 39,
@@ -273,10 +274,10 @@ vbm_status vbm_weighted_combine(const float * y, const float * weights, int64_t 
                                 int64_t n_ids, int64_t n_tokens, float * out, void * stream);
 
 /* ----------------------------------------------------------------------------------------------
- * Block-scaled FP8 and 16-bit products, for checkpoints whose weights are kept as they are stored:
- * row-major matrices of e4m3 codes with one fp32 scale per 128 x 128 block, or of fp16 / bf16. No
- * counterpart in the reference (its expert weights are ggml-quantized); they take the router's, the
- * grouping's and the combine's buffers as the calls above leave them:
+ * Block-scaled FP8, 8-bit integer and 16-bit products, for checkpoints whose weights are kept as they are
+ * stored: row-major matrices of e4m3 codes with one fp32 scale per 128 x 128 block, of 8-bit integers with one
+ * per row (output channel), or of fp16 / bf16. No counterpart in the reference (its expert weights are
+ * ggml-quantized); they take the router's, the grouping's and the combine's buffers as the calls above leave them:
  *
  *   vbm_router_topk_softmax -> ids, weights
  *   vbm_group_by_expert     -> offsets, rows
@@ -285,6 +286,9 @@ vbm_status vbm_weighted_combine(const float * y, const float * weights, int64_t 
  *   vbm_glu_quantize_fp8    gate | up halves -> codes, scales, grouped
  *   vbm_grouped_mul_mat     down: dst_rows = rows -> y [n_tokens][top_k][H] (F32)
  *   vbm_weighted_combine    y, weights -> out [n_tokens][H]
+ *
+ * and with integers the same with vbm_quantize_i8 and vbm_glu_quantize_i8. vbm_add_rms_norm_quantize takes the place of the
+ * first quantizer where the rows come from a residual stream: its y is what the router reads.
  *
  * The down product does not write the rows of y whose ids are -1 (the grouping skips them), and the combine reads all of y: where
  * there can be such ids, vbm_memset y to 0 before it (their weights should be 0 too).
@@ -307,11 +311,35 @@ vbm_status vbm_glu_quantize_fp8(int activation, int x_type, const void * gate, c
                                 int64_t width, int64_t gate_stride, int64_t up_stride, float alpha, float limit,
                                 void * codes, float * scales, void * stream);
 
+/* Rows of x (as vbm_quantize_fp8; k at most 65536) -> 8-bit integers [n_rows][k] (16-byte aligned) and fp32 scales [n_rows]. For a
+ * row with a = max(max |x|, 2^-116): scale = a / 127, code = 127 x / a to the nearest integer, ties to even: 127 x rounded to fp32 (exact
+ * for F16 and BF16), its quotient by a correctly rounded to fp32, and that to an integer, -127..127. A row that holds a NaN or an infinity gets the
+ * scale NaN and zero codes. n_rows = 0 does nothing. */
+vbm_status vbm_quantize_i8(int x_type, const void * x, int64_t n_rows, int64_t k, int64_t x_stride, void * codes, float * scales,
+                           void * stream);
+/* act(gate, up) as in vbm_glu_quantize_fp8, quantized as by vbm_quantize_i8. */
+vbm_status vbm_glu_quantize_i8(int activation, int x_type, const void * gate, const void * up, int64_t n_rows, int64_t width,
+                               int64_t gate_stride, int64_t up_stride, float alpha, float limit, void * codes, float * scales,
+                               void * stream);
+
+/* A block's output added to the residual stream, the root-mean-square norm of the sum, and its 8-bit codes, in one pass:
+ *   s = x + residual, rounded to x_type     v = s / sqrt(mean(s^2) + eps) * weight, in fp32
+ * over rows of k values (a multiple of 16, at most 65536). x and residual are of x_type (F32, F16 or BF16), rows x_stride and
+ * residual_stride elements apart. residual may be NULL (s = x). sum, if given, gets s, laid out as residual; it may be the
+ * residual's own buffer, or x's where both strides agree. weight [k] fp32 or NULL (ones). y, if given, gets v rounded to y_type,
+ * [n_rows][k]. codes (16-byte aligned), if given, [n_rows][k] of code_type: VBM_TYPE_F8_E4M3 with scales [n_rows][ceil(k / 128)] as
+ * vbm_quantize_fp8 makes them of v, or VBM_TYPE_I8 with scales [n_rows] as vbm_quantize_i8 does. At least one of y and codes; eps > 0. A
+ * row whose sum of squares is no fp32 number (a NaN, an infinity, or values that large) comes out as NaN: y NaN, scales NaN and
+ * codes zero; its sum is stored as it is. n_rows = 0 does nothing. */
+vbm_status vbm_add_rms_norm_quantize(int x_type, const void * x, int64_t x_stride, const void * residual, void * sum,
+                                     int64_t residual_stride, const float * weight, int64_t n_rows, int64_t k, float eps, int y_type,
+                                     void * y, int code_type, void * codes, float * scales, void * stream);
+
 /* n_groups weight matrices [rows][k], one after the other (device memory, 16-byte aligned). */
 typedef struct vbm_weights {
-    int type;                      /* VBM_TYPE_F8_E4M3 (k % 16 == 0), VBM_TYPE_F16 or VBM_TYPE_BF16 (k % 8 == 0) */
+    int type;                      /* VBM_TYPE_F8_E4M3 or VBM_TYPE_I8 (k % 16 == 0), VBM_TYPE_F16 or VBM_TYPE_BF16 (k % 8 == 0) */
     const void * data;             /* [n_groups][rows][k]                                        */
-    const float * scales;          /* F8: [n_groups][ceil(rows / 128)][ceil(k / 128)], else unused */
+    const float * scales;          /* F8: [n_groups][ceil(rows / 128)][ceil(k / 128)], I8: [n_groups][rows], else unused */
     const float * bias;            /* [n_groups][rows] or NULL                                   */
     int64_t n_groups;              /* 1..1024                                                    */
     int64_t rows, k;
@@ -326,12 +354,20 @@ typedef struct vbm_weights {
 vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type,
                            void * dst, void * stream);
 
+/* dst[t][n] = (w.scales[n] * b_scales[t]) * (w[n] . b[t]) (+ bias[n]) of one matrix of 8-bit integers (-128..127; k < 131072) with tokens
+ * quantized by vbm_quantize_i8: b [n_tokens][k] (16-byte aligned), b_scales [n_tokens], dst [n_tokens][rows] of dst_type (F32, F16 or
+ * BF16); n_tokens < 2^29. The integer sums are exact; they, the product of the two scales, its product with the sum and the
+ * bias's addition are each rounded to fp32, and the result to dst_type. n_tokens = 0 does nothing. */
+vbm_status vbm_mul_mat_i8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type, void * dst,
+                          void * stream);
+
 /* The products of rows grouped by expert, with any number of rows a group: for every group g and i in
  * [offsets[g], offsets[g + 1]),
  *   dst[dst_rows ? dst_rows[i] : i] = w[g] . b[b_rows ? b_rows[i] / b_div : i] (+ bias[g])
  * offsets [n_groups + 1] as vbm_group_by_expert writes them, n_rows >= offsets[n_groups] the most rows there
  * can be (its n_ids * n_tokens), by whose mean a group the kernel is chosen; neither is read on the host. b is [n_b][k] (n_b > 0) in the weights' type (F8: codes with
- * b_scales [n_b][ceil(k / 128)]), dst [n_dst][rows] of dst_type; sums as in vbm_mul_mat_fp8 (its tokens: n_rows / n_groups). A b row outside [0, n_b) makes its outputs NaN; a dst
+ * b_scales [n_b][ceil(k / 128)], I8: with b_scales [n_b]), dst [n_dst][rows] of dst_type; sums as in vbm_mul_mat_fp8 (its tokens: n_rows / n_groups)
+ * and vbm_mul_mat_i8. A b row outside [0, n_b) makes its outputs NaN; a dst
  * row outside [0, n_dst) is not written, nor are dst rows that no group lists. dst_rows must not list a
  * row twice. n_rows < 2^29; n_rows = 0 does nothing. */
 vbm_status vbm_grouped_mul_mat(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_b,

@@ -1,11 +1,13 @@
 // Products of weight matrices with token rows, dense or grouped by expert: FP8 (e4m3) weights with one fp32 scale per
-// 128 x 128 block and activations with one per 128 values of a row, or fp16 / bf16 weights and activations.
+// 128 x 128 block and activations with one per 128 values of a row, 8-bit integer weights and activations with one fp32 scale per
+// row, or fp16 / bf16 weights and activations.
 //
-//   FP8:    dst[t][n] = sum over blocks kb of ws[n / 128][kb] * bs[t][kb] * (sum over the block's k of w[n][k] b[t][k])
-//   16-bit: dst[t][n] = sum over k of w[n][k] b[t][k]
+//   FP8:      dst[t][n] = sum over blocks kb of ws[n / 128][kb] * bs[t][kb] * (sum over the block's k of w[n][k] b[t][k])
+//   integers: dst[t][n] = (ws[n] * bs[t]) * (sum over k of w[n][k] b[t][k]), the sum exact in 32 bits (k < 2^17)
+//   16-bit:   dst[t][n] = sum over k of w[n][k] b[t][k]
 //
 // plus a bias. Everything is laid out along k, so the kernels see rows of bytes and take 128 of them a step: one FP8 scale
-// block, or 64 16-bit values. As a matrix operand lane (q, r) = (lane / 16, lane % 16) holds 32 of row r's 128 bytes; which ones
+// block, 128 integers, or 64 16-bit values. As a matrix operand lane (q, r) = (lane / 16, lane % 16) holds 32 of row r's 128 bytes; which ones
 // does not matter as long as both operands agree. The weights are the A operand and the tokens B, so that a lane's four results
 // are four neighbouring outputs of one token.
 #include <algorithm>
@@ -19,6 +21,7 @@ namespace vbm {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4p __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2p __attribute__((ext_vector_type(2)));
@@ -28,10 +31,10 @@ typedef __bf16 bf16x8_p __attribute__((ext_vector_type(8)));
 
 struct ProductArgs {
     const uint8_t * w;             // [n_groups][rows][k_bytes]
-    const float * ws;              // [n_groups][ceil(rows / 128)][kb], FP8 only
+    const float * ws;              // FP8 [n_groups][ceil(rows / 128)][kb], integers [n_groups][rows]
     const float * bias;            // [n_groups][rows] or null
     const uint8_t * b;             // [n_b][k_bytes]
-    const float * bs;              // [n_b][kb], FP8 only
+    const float * bs;              // FP8 [n_b][kb], integers [n_b]
     int64_t n_b;
     const int32_t * b_rows;        // grouped row -> b row times b_div, or null (b row = grouped row)
     int64_t b_div;
@@ -188,11 +191,11 @@ __device__ __forceinline__ half8_p widened(unsigned a, unsigned b) {
     return half8_p{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
 
-// A piece as matrix operands, and the product of two of them added to c.
+// A piece as matrix operands, and the product of two of them added to c (integers: the bits of 32-bit ones).
 template <int KIND>
 struct Operand {
     static constexpr int N = KIND == kF8 ? 1 : (KIND == kF8Wide ? 4 : 2);
-    using T = std::conditional_t<KIND == kF8, i32x8, std::conditional_t<KIND == kBF16, bf16x8_p, half8_p>>;
+    using T = std::conditional_t<KIND == kF8, i32x8, std::conditional_t<KIND == kI8, i32x4, std::conditional_t<KIND == kBF16, bf16x8_p, half8_p>>>;
     T v[N];
     __device__ __forceinline__ void take(const Piece & p) {
         if constexpr (KIND == kF8) {
@@ -209,11 +212,35 @@ template <int KIND>
 __device__ __forceinline__ f32x4 product(const Operand<KIND> & a, const Operand<KIND> & b, f32x4 c) {
 #pragma unroll
     for (int i = 0; i < Operand<KIND>::N; ++i) {
-        if constexpr (KIND == kF8) c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v[i], b.v[i], c, 0, 0, 0, 0, 0, 0);
+        if constexpr (KIND == kI8) c = __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(a.v[i], b.v[i], __builtin_bit_cast(i32x4, c), 0, 0, 0));
+        else if constexpr (KIND == kF8) c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v[i], b.v[i], c, 0, 0, 0, 0, 0, 0);
         else if constexpr (KIND == kBF16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
         else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[i], b.v[i], c, 0, 0, 0);
     }
     return c;
+}
+// Sums of products added up, and as outputs: of integers times the scales of their rows and their token.
+template <int KIND>
+__device__ __forceinline__ f32x4 joined(f32x4 a, f32x4 b) {
+    if constexpr (KIND == kI8) return __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, a) + __builtin_bit_cast(i32x4, b));
+    return a + b;
+}
+template <int KIND>
+__device__ __forceinline__ f32x4 scaled(f32x4 sum, f32x4 row_scales, float token_scale) {
+    if constexpr (KIND != kI8) return sum;
+    const i32x4 n = __builtin_bit_cast(i32x4, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = static_cast<float>(n[e]) * (row_scales[e] * token_scale);
+    return sum;
+}
+// Values n .. n + 3 of a group's row of `rows` values; zeros past the end or without a row.
+__device__ __forceinline__ f32x4 row_values(const ProductArgs & A, const float * p, int group, int n) {
+    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!p) return v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < A.rows) v[e] = p[static_cast<int64_t>(group) * A.rows + n + e];
+    return v;
 }
 
 // Loads from memory to LDS (lane l's bytes land at m0 + l * size), in inline assembly so that the compiler does not wait for
@@ -303,7 +330,12 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
         const float * ssrc = is_f8(KIND) ? A.bs + token_row(lane >> 2) * A.kb : nullptr;
         // piece lane % 8 of a row sits at its place xor (row / 2 % 8), as in the kernels below
         const int piece_even = (lane & 7) ^ (lane >> 4), piece_odd = piece_even ^ 4;
-        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f}, row_scales{0.0f, 0.0f, 0.0f, 0.0f};
+        float token_scale = 0.0f;
+        if constexpr (KIND == kI8) {                         // (asked for here, so that nobody waits for them at the end)
+            row_scales = row_values(A, A.ws, t.group, n0 + 4 * q);
+            token_scale = A.bs[token_row(r)];
+        }
 
         for (int k0 = k_begin; k0 < k_end; k0 += RUN) {
             const int n_steps = k_end - k0 < RUN ? k_end - k0 : RUN;
@@ -372,17 +404,14 @@ __global__ __launch_bounds__(256) void few_rows_kernel(ProductArgs A, int row_ti
         if (wave) return;
         f32x4 v = parts[lane];
 #pragma unroll
-        for (int w = 1; w < W; ++w) v += parts[w * 64 + lane];
+        for (int w = 1; w < W; ++w) v = joined<KIND>(v, parts[w * 64 + lane]);
+        v = scaled<KIND>(v, row_scales, token_scale);
         const int n = n0 + 4 * q;
         const int64_t i = t.first + r;
         if (i >= t.last || n >= A.rows) return;
         const int64_t row = target_row(A, i);
         if (row < 0) return;
-        if (A.bias) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < A.rows) v[e] += A.bias[static_cast<int64_t>(t.group) * A.rows + n + e];
-        }
+        if (A.bias) v += row_values(A, A.bias, t.group, n);
         const float nan = __builtin_nanf("");
         store4(A, row, n, source_row(A, i) < 0 ? f32x4{nan, nan, nan, nan} : v);
     };
@@ -473,9 +502,13 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
             load_to_lds_4(A.ws + (static_cast<int64_t>(t.group) * blocks + block) * A.kb + (lane < A.kb ? lane : A.kb - 1), lds0 + L::BLOCK_SCALES + i * 256);
         }
     }
-    float * bias = reinterpret_cast<float *>(lds + L::BIAS);
-    for (int i = threadIdx.x; i < W * 16 * tiles; i += W * 64)
+    float * bias = reinterpret_cast<float *>(lds + L::BIAS), * row_scales = reinterpret_cast<float *>(lds + L::BLOCK_SCALES);
+    for (int i = threadIdx.x; i < W * 16 * tiles; i += W * 64) {
         bias[i] = A.bias && n0 + i < A.rows ? A.bias[static_cast<int64_t>(t.group) * A.rows + n0 + i] : 0.0f;
+        if constexpr (KIND == kI8) row_scales[i] = n0 + i < A.rows ? A.ws[static_cast<int64_t>(t.group) * A.rows + n0 + i] : 0.0f;
+    }
+    float token_scale = 0.0f;
+    if constexpr (KIND == kI8) token_scale = A.bs[token_row(r)];
     const int64_t mine = t.first + r, to = mine < t.last ? target_row(A, mine) : -1;   // the dst row of token r; -1: none
     const bool bad = to >= 0 && source_row(A, mine) < 0;
     landed<0>();
@@ -520,6 +553,7 @@ __global__ __launch_bounds__(W * 64) void stream_rows_kernel(ProductArgs A, int 
                 slot = slot + 1 == D ? 0 : slot + 1;
             }
             const f32x4 extra = *reinterpret_cast<const f32x4 *>(bias + (n - n0) + 4 * q);
+            if constexpr (KIND == kI8) acc = scaled<KIND>(acc, *reinterpret_cast<const f32x4 *>(row_scales + (n - n0) + 4 * q), token_scale);
             const float nan = __builtin_nanf("");
             if (to >= 0 && n + 4 * q < A.rows) store4(A, to, n + 4 * q, bad ? f32x4{nan, nan, nan, nan} : acc + extra);
         }
@@ -651,7 +685,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;
     constexpr int DW = BN / 8 / W;                           // a wave's loads of weights a step: 8 rows each
     static_assert(DW * 8 * W == BN && BT % 32 == 0, "the waves share the loads");
-    constexpr int STAGE_BYTES = LDS - BT * 4;
+    constexpr int STAGE_BYTES = LDS - BT * (KIND == kI8 ? 8 : 4);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
     Work work;
     if (!find_work(A, ST * WT, row_tiles, launched, work)) return;
@@ -686,6 +720,10 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         const int64_t i = static_cast<int64_t>(work.first) + c;
         const int row = c < work.live ? static_cast<int>(target_row(A, i)) : -1;
         rows[c] = row >= 0 && source_row(A, i) < 0 ? -2 - row : row;
+    }
+    float * token_scales = reinterpret_cast<float *>(lds + STAGE_BYTES + BT * 4);   // of integers
+    if constexpr (KIND == kI8) {
+        for (int c = threadIdx.x; c < BT; c += W * 64) token_scales[c] = A.bs[token_row(c)];
     }
 
     const int live_cols = (work.live + 15) >> 4;
@@ -855,19 +893,19 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         constexpr int ROW = 16 * SN * 4 + 16;                // bytes of a token's outputs there
         static_assert(W * 16 * ROW <= STAGE_BYTES, "the stages' memory holds them");
         const int nw = n0 + 16 * SN * wn;                    // the wave's first output
-        f32x4 bias[SN];
+        f32x4 bias[SN], row_scales[SN];
 #pragma unroll
-        for (int s = 0; s < SN; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = nw + 16 * s + 4 * q + e;
-                bias[s][e] = A.bias && n < A.rows ? A.bias[static_cast<int64_t>(work.group) * A.rows + n] : 0.0f;
-            }
+        for (int s = 0; s < SN; ++s) {
+            bias[s] = row_values(A, A.bias, work.group, nw + 16 * s + 4 * q);
+            row_scales[s] = KIND == kI8 ? row_values(A, A.ws, work.group, nw + 16 * s + 4 * q) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
         uint8_t * mine = lds + wave * 16 * ROW;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+            const float token_scale = KIND == kI8 ? token_scales[16 * (j * WT + wt) + r] : 0.0f;
 #pragma unroll
-            for (int s = 0; s < SN; ++s) *reinterpret_cast<f32x4 *>(mine + r * ROW + 64 * s + 16 * q) = acc[s][j] + bias[s];
+            for (int s = 0; s < SN; ++s)
+                *reinterpret_cast<f32x4 *>(mine + r * ROW + 64 * s + 16 * q) = scaled<KIND>(acc[s][j], row_scales[s], token_scale) + bias[s];
             const int * to = rows + 16 * (j * WT + wt);
             if (A.dst_type == VBM_TYPE_F32) store_column<4 * SN, 4>(A, mine, ROW, to, nw);
             else store_column<2 * SN, 8>(A, mine, ROW, to, nw);
@@ -948,17 +986,18 @@ void launch_product(const ProductArgs & a, hipStream_t stream) {
 }
 
 void product(const vbm_weights & w, const void * b, const float * b_scales, ProductArgs a, int dst_type, void * dst, hipStream_t stream) {
-    const bool f8 = w.type == VBM_TYPE_F8_E4M3;
-    require(f8 || w.type == VBM_TYPE_F16 || w.type == VBM_TYPE_BF16, "weights must be F8_E4M3, F16 or BF16");
+    const bool f8 = w.type == VBM_TYPE_F8_E4M3, i8 = w.type == VBM_TYPE_I8, bytes = f8 || i8;
+    require(bytes || w.type == VBM_TYPE_F16 || w.type == VBM_TYPE_BF16, "weights must be I8, F8_E4M3, F16 or BF16");
     require(dst_type == VBM_TYPE_F32 || dst_type == VBM_TYPE_F16 || dst_type == VBM_TYPE_BF16, "dst must be F32, F16 or BF16");
     require(w.n_groups > 0 && w.n_groups <= 1024, "n_groups must be in 1..1024");
     require(w.rows > 0 && w.rows < (int64_t{1} << 30) && w.k > 0 && w.k < (int64_t{1} << 23), "rows and k out of range");
-    const int64_t k_bytes = w.k * (f8 ? 1 : 2);
-    require(k_bytes % 16 == 0, f8 ? "k must be a multiple of 16" : "k must be a multiple of 8");
+    require(!i8 || w.k < (int64_t{1} << 17), "k of integers must be less than 131072");
+    const int64_t k_bytes = w.k * (bytes ? 1 : 2);
+    require(k_bytes % 16 == 0, bytes ? "k must be a multiple of 16" : "k must be a multiple of 8");
     require(a.n_rows >= 0 && a.n_rows < (int64_t{1} << 29) && a.n_b >= 0 && a.n_dst >= 0 && a.n_dst < (int64_t{1} << 31) - 2, "row counts out of range");
     require(a.b_div > 0 && a.b_div < (int64_t{1} << 31), "b_div must be positive");
     if (a.n_rows == 0) return;
-    require(w.data && b && dst && a.n_b > 0 && (!f8 || (w.scales && b_scales)), "null buffer");
+    require(w.data && b && dst && a.n_b > 0 && (!bytes || (w.scales && b_scales)), "null buffer");
     auto at = [](const void * p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
     require(at(w.data, 16) && at(b, 16), "weights and b must be 16-byte aligned");
     const size_t dsize = dst_type == VBM_TYPE_F32 ? 4 : 2;
@@ -979,6 +1018,7 @@ void product(const vbm_weights & w, const void * b, const float * b_scales, Prod
     a.kb = static_cast<int>((k_bytes + 127) / 128);
     if (f8 && dst_type == VBM_TYPE_BF16) launch_product<kF8>(a, stream);
     else if (f8) launch_product<kF8Wide>(a, stream);
+    else if (i8) launch_product<kI8>(a, stream);
     else if (w.type == VBM_TYPE_F16) launch_product<kF16>(a, stream);
     else launch_product<kBF16>(a, stream);
 }
@@ -995,6 +1035,18 @@ vbm_status vbm_mul_mat_fp8(const vbm_weights * w, const void * b, const float * 
     return guarded([&] {
         require(w != nullptr, "null weights");
         require(w->type == VBM_TYPE_F8_E4M3 && w->n_groups == 1, "weights must be one F8_E4M3 matrix");
+        ProductArgs a{};
+        a.n_b = a.n_rows = a.n_dst = n_tokens;
+        a.b_div = 1;
+        product(*w, b, b_scales, a, dst_type, dst, as_stream(stream));
+    });
+}
+
+vbm_status vbm_mul_mat_i8(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_tokens, int dst_type, void * dst,
+                          void * stream) {
+    return guarded([&] {
+        require(w != nullptr, "null weights");
+        require(w->type == VBM_TYPE_I8 && w->n_groups == 1, "weights must be one I8 matrix");
         ProductArgs a{};
         a.n_b = a.n_rows = a.n_dst = n_tokens;
         a.b_div = 1;

@@ -17,7 +17,8 @@ namespace vbm {
 //        1536 x 2048 123 against 156. Up to 10 rows a group both take as long: one token through 8 experts 9.2 (7.1 against 6.6 with the
 //        weights in the caches), 64 tokens top-4 over 32 experts of 5760 x 2880 103 and 104. An fp16 output's rounding, 2e-4, would not cover it.
 //   kF16, kBF16: as they are.
-enum Kind { kF8Wide, kF8, kF16, kBF16 };
+//   kI8: 8-bit integers, by the integer matrix instruction, at the FP8 one's rate: exact products and sums.
+enum Kind { kF8Wide, kF8, kF16, kBF16, kI8 };
 constexpr bool is_f8(int kind) { return kind == kF8Wide || kind == kF8; }
 
 // LDS of the streaming kernel (W waves, tokens by MAX8 eights, rings of D steps).
@@ -27,7 +28,7 @@ struct StreamLayout {
     static constexpr int MAX_TILES = 4;
     static constexpr int TOTAL = W * 20 * 1024;              // two workgroups of 4 waves, or one of 8, a CU
     static constexpr int RING = W * D * 2048, ROWS = W * MAX_TILES * 16, BLOCKS = ROWS / 128 + 2;
-    static constexpr int BIAS = RING, BLOCK_SCALES = BIAS + ROWS * 4, TOKENS = BLOCK_SCALES + (is_f8(KIND) ? BLOCKS * 256 : 0);
+    static constexpr int BIAS = RING, BLOCK_SCALES = BIAS + ROWS * 4, TOKENS = BLOCK_SCALES + (is_f8(KIND) ? BLOCKS * 256 : (KIND == kI8 ? ROWS * 4 : 0));   // (integers: a scale per row there)
     static constexpr int STEP = MAX8 * 1024 + (is_f8(KIND) ? 64 : 0);   // a step of the tokens and their scales
     // steps that fit (scales come in fours; the weights' scales of 64 steps are kept)
     static constexpr int FIT = (TOTAL - TOKENS - (is_f8(KIND) ? 4 * 64 : 0)) / STEP;
