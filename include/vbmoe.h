@@ -289,6 +289,7 @@ vbm_status vbm_weighted_combine(const float * y, const float * weights, int64_t 
  *
  * and with integers the same with vbm_quantize_i8 and vbm_glu_quantize_i8. vbm_add_rms_norm_quantize takes the place of the
  * first quantizer where the rows come from a residual stream: its y is what the router reads.
+ * For up to 16 tokens vbm_moe_few_forward does all of it from the logits on.
  *
  * The down product does not write the rows of y whose ids are -1 (the grouping skips them), and the combine reads all of y: where
  * there can be such ids, vbm_memset y to 0 before it (their weights should be 0 too).
@@ -373,6 +374,30 @@ vbm_status vbm_mul_mat_i8(const vbm_weights * w, const void * b, const float * b
 vbm_status vbm_grouped_mul_mat(const vbm_weights * w, const void * b, const float * b_scales, int64_t n_b,
                                const int32_t * b_rows, int64_t b_div, const int32_t * offsets, int64_t n_rows,
                                const int32_t * dst_rows, int64_t n_dst, int dst_type, void * dst, void * stream);
+
+/* A routed-expert layer for a few tokens (up to 16, and up to 128 (token, rank) pairs) over weights as they are stored, in two launches:
+ *   out[t] = sum over ranks r of weights[t][r] * (down[e] act(gate_up[e] x[t] + its bias) + its bias),  e = ids[t][r]
+ * in the ranks' order. The activations are not quantized: x is taken as it is, F8 and I8 weights times their scales, and everything between
+ * is held in fp32 (all products exact in fp32, fp32 sums); only out is rounded to its type. So results are nearer to the formula than those of the
+ * chain above, which rounds the activations to 8 bits twice. */
+typedef struct vbm_moe_few_desc {
+    vbm_weights gate_up;           /* [n_experts][2 * I][H]: rows [0, I) gate, [I, 2 * I) up; with bias or not  */
+    vbm_weights down;              /* [n_experts][H][I], of gate_up's type                      */
+    int64_t top_k;                 /* 1..64                                                     */
+    int activation;                /* VBM_ACT_*, with alpha and limit as in vbm_glu             */
+    float alpha, limit;
+} vbm_moe_few_desc;
+
+vbm_status vbm_moe_few_workspace(const vbm_moe_few_desc * desc, int64_t n_tokens, size_t * bytes);
+
+/* x [n_tokens][H] of x_type (F32, F16 or BF16; 16-byte aligned) -> out [n_tokens][H] of out_type (F32, F16 or BF16; it may be x's buffer).
+ * logits [n_tokens][n_experts] fp32: each token's top_k and the softmax over them, as vbm_router_topk_softmax chooses them; ids and weights
+ * [n_tokens][top_k], where given, receive them. logits NULL: ids and weights are the routing. There an id of -1 adds nothing, any other outside
+ * [0, n_experts) makes its token's outputs NaN, and an expert may be listed more than once. An infinity or a NaN in x makes its token's outputs NaN.
+ * `workspace`: 16-byte aligned device memory of the size above; it holds nothing between calls, and calls that share one must not overlap.
+ * Can be captured. A call repeated on the same inputs gives the same bits. n_tokens = 0 does nothing. */
+vbm_status vbm_moe_few_forward(const vbm_moe_few_desc * desc, int x_type, const void * x, const float * logits, int32_t * ids, float * weights,
+                               int64_t n_tokens, int out_type, void * out, void * workspace, size_t workspace_bytes, void * stream);
 
 /* ----------------------------------------------------------------------------------------------
  * Fused routed-expert layer (expert_branch of hybrid-experts.patch:1394-1683 for one layer:

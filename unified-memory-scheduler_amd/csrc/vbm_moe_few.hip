@@ -1,0 +1,730 @@
+// A routed-expert layer for a few tokens, weights as they are stored, in two launches:
+//
+//   h[t, r] = act(Wg[e] x[t] + bg[e], Wu[e] x[t] + bu[e])            e = ids[t, r]
+//   out[t]  = sum over ranks r of weights[t, r] * (Wd[e] h[t, r] + bd[e])
+//
+// The first launch routes (top-k of the logits and the softmax over it, every workgroup for itself) and makes h, the second multiplies
+// by the down weights and adds the ranks up, in their order. What such a step has to do is read the touched experts' weights once; the kernels
+// differ from the grouped products in what they save around that: five launches, and the rows between them.
+//
+// The activations are not quantized. The weights are widened to bf16, exactly (e4m3 has 4 significant bits, 8-bit integers have 8; fp16's 11
+// are two bf16 values), and so are the activations, as sums of bf16 values: fp32 ones of three (8 + 8 + 8 bits, each the leading
+// bits of what is left, so the last one is exact), fp16 of two, bf16 of one. Each term is a column of the matrix instruction's B operand, whose
+// 16 columns a few tokens would leave unused anyway: 5 rows of three terms or 8 of one or two. All products are exact in fp32, as in an fp32
+// program, and summed in fp32; h is kept as its three terms. An infinity or NaN in x makes its token's outputs NaN.
+//
+// Rows are grouped by expert into slots of up to as many (token, rank) entries as there are columns, in the order in which they first
+// appear; every wave finds its slot by itself from the ids: with ten ballots each lane knows the entries of its entry's expert.
+// The weights stream as in the grouped products: 16 rows by 128 bytes a step, loaded straight to a ring in LDS of each wave, with the
+// activations of the step behind them (they come from the L2, and the waits count all loads alike).
+#include <algorithm>
+#include <type_traits>
+
+#include "vbm_device.hpp"
+#include "vbm_internal.hpp"
+#include "vbm_lds_stream.hpp"
+#include "vbm_quantize.hpp"
+
+namespace vbm {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMostTokens = 16, kMostEntries = 128;
+constexpr int kTerms = -1;                     // the type of h: three bf16 terms of each value, a step's first, second, third
+
+constexpr bool one_byte(int kind) { return kind == VBM_TYPE_F8_E4M3 || kind == VBM_TYPE_I8; }
+
+// A step's activations of one entry.
+template <int KIND, int X>
+struct Rows {
+    static constexpr int VALUES = one_byte(KIND) ? 128 : 64;                      // of k, a step
+    static constexpr int TERMS = X == VBM_TYPE_BF16 ? 1 : (X == VBM_TYPE_F16 ? 2 : 3);
+    static constexpr int MOST = TERMS < 3 ? 8 : (X == kTerms && one_byte(KIND) ? 4 : 5);   // entries a slot: (the fifth's pieces take a fourth load)
+    static constexpr int BYTES = VALUES * (X == kTerms ? 6 : (X == VBM_TYPE_F32 ? 4 : 2)), PIECES = BYTES / 16;
+    static constexpr int loads(int entries) { return (entries * PIECES + 63) / 64; }   // of a wave, 64 pieces each
+};
+
+struct FewArgs {
+    const uint8_t * w;             // [n_expert][rows][k_bytes]
+    const float * ws, * bias;      // as vbm_weights has them
+    const void * x;                // x [n_tokens][k], or h [entries][kb][three terms of a step]
+    const int32_t * ids;           // [entries]
+    const float * logits;          // or null: then ids are read
+    int32_t * ids_out;             // with logits
+    float * weights_out;
+    const float * weights;         // [entries], the second launch's
+    uint8_t * h;                   // the first launch's outputs
+    void * out;
+    int out_type;
+    int n_tokens, top_k, n_expert, entries, capacity;   // capacity: most entries a slot
+    int rows, k_bytes, kb;         // of this launch's matrix
+    int inter, h_kb, h_step;       // I; steps of a row of h, and their bytes
+    int row_units, tiles;          // workgroups a slot; row tiles a wave
+    int activation;
+    float alpha, limit;
+};
+
+// The entries' grouping by expert, as every wave finds it: lane l holds entries l and 64 + l.
+struct Slots {
+    int id[2], position[2];        // of the entry among those of its expert
+    uint64_t same[2][2];           // the entries of its expert
+    uint64_t leads[2];             // entries that begin a slot
+    __device__ __forceinline__ Slots(const int32_t * ids, int entries, int n_expert, int capacity) {
+        const int lane = threadIdx.x & 63;
+        const uint64_t below = (uint64_t{1} << lane) - 1;
+        uint64_t valid[2], plane[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            id[s] = lane + 64 * s < entries ? ids[lane + 64 * s] : -1;
+            if (static_cast<unsigned>(id[s]) >= static_cast<unsigned>(n_expert)) id[s] = -1;
+            valid[s] = __ballot(id[s] >= 0);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) same[s][o] = valid[o];
+#pragma unroll
+        for (int b = 0; b < 10; ++b) {
+#pragma unroll
+            for (int o = 0; o < 2; ++o) plane[o] = __ballot(id[o] >> b & 1);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int o = 0; o < 2; ++o) same[s][o] &= id[s] >> b & 1 ? plane[o] : ~plane[o];
+        }
+        position[0] = __popcll(same[0][0] & below);
+        position[1] = __popcll(same[1][0]) + __popcll(same[1][1] & below);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) leads[s] = __ballot(id[s] >= 0 && position[s] % capacity == 0);
+    }
+    __device__ __forceinline__ int count() const { return __popcll(leads[0]) + __popcll(leads[1]); }
+    // The number of the slot that entry (s, this lane) begins.
+    __device__ __forceinline__ int number(int s) const {
+        const uint64_t below = (uint64_t{1} << (threadIdx.x & 63)) - 1;
+        return s ? __popcll(leads[0]) + __popcll(leads[1] & below) : __popcll(leads[0] & below);
+    }
+    // Slot `index`: its expert, and its entries into list[]; their number.
+    __device__ __forceinline__ int find(int index, int capacity, int & expert, int * list) const {
+        const int lane = threadIdx.x & 63;
+        int first = 0, n = 0;
+        expert = -1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint64_t at = __ballot((leads[s] >> lane & 1) && number(s) == index);
+            if (!at) continue;
+            const int l = __builtin_ctzll(at);
+            expert = __builtin_amdgcn_readlane(id[s], l);
+            first = __builtin_amdgcn_readlane(position[s], l);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const bool mine = expert >= 0 && id[s] == expert && position[s] >= first && position[s] < first + capacity;
+            if (mine) list[position[s] - first] = lane + 64 * s;
+            n += __popcll(__ballot(mine));
+        }
+        return n;
+    }
+    // All slots: experts, numbers of entries, entries [slot][capacity]. By one wave.
+    __device__ __forceinline__ void table(int capacity, int * experts, int * counts, int * list) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (id[s] < 0) continue;
+            uint64_t m0 = same[s][0], m1 = same[s][1];
+            const int total = __popcll(m0) + __popcll(m1), first = position[s] / capacity * capacity;
+            for (int j = 0; j < first; ++j) {                // (the first entry of its slot: a slot holds almost always all of them)
+                if (m0) m0 &= m0 - 1;
+                else m1 &= m1 - 1;
+            }
+            const uint64_t below = (uint64_t{1} << __builtin_ctzll(m0 ? m0 : m1)) - 1;
+            const int slot = m0 ? __popcll(leads[0] & below) : __popcll(leads[0]) + __popcll(leads[1] & below);
+            list[slot * capacity + position[s] - first] = lane + 64 * s;
+            if (position[s] == first) {
+                experts[slot] = id[s];
+                counts[slot] = total - first < capacity ? total - first : capacity;
+            }
+        }
+    }
+};
+
+// ids (and weights) of the tokens into LDS, by top-k of the logits or from the caller; W waves.
+template <int W>
+__device__ __forceinline__ void route(const FewArgs & A, int32_t * ids, bool writes) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (!A.logits) {
+        for (int i = threadIdx.x; i < A.entries; i += W * 64) ids[i] = A.ids[i];
+        return;
+    }
+    auto pick = [&](auto npl_c) {
+        constexpr int NPL = decltype(npl_c)::value;
+        for (int t = wave; t < A.n_tokens; t += W) {
+            float lg[NPL], value;
+            int id;
+#pragma unroll
+            for (int c = 0; c < NPL; ++c) lg[c] = lane + 64 * c < A.n_expert ? route_key(A.logits[static_cast<int64_t>(t) * A.n_expert + lane + 64 * c]) : 0.0f;
+            wave_topk_regs<NPL>(lg, A.n_expert, A.top_k, value, id);
+            if (lane < A.top_k) ids[t * A.top_k + lane] = id;
+            if (writes) {
+                const float w = wave_pick_softmax(value, A.top_k);
+                if (lane < A.top_k) {
+                    A.ids_out[t * A.top_k + lane] = id;
+                    A.weights_out[t * A.top_k + lane] = w;
+                }
+            }
+        }
+    };
+    if (A.n_expert <= 128) pick(std::integral_constant<int, 2>{});
+    else if (A.n_expert <= 256) pick(std::integral_constant<int, 4>{});
+    else pick(std::integral_constant<int, 16>{});
+}
+
+__device__ __forceinline__ unsigned upper_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302u);
+}
+__device__ __forceinline__ float without(float v, unsigned mask) {   // v minus the bits of it that `mask` keeps
+    return v - __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & mask);
+}
+
+// Eight weights as bf16 values; fp16's upper parts, and what is left of them in `rest`.
+template <int KIND>
+__device__ __forceinline__ bf16x8 widened(const unsigned * w, bf16x8 & rest) {
+    if constexpr (KIND == VBM_TYPE_BF16) {
+        return __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
+    } else if constexpr (KIND == VBM_TYPE_F8_E4M3) {
+        const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.0f, true);
+        const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.0f, true);
+        return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+    } else if constexpr (KIND == VBM_TYPE_I8) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned two = w[i >> 1] >> (16 * (i & 1));
+            v[i] = upper_halves(static_cast<float>(static_cast<int8_t>(two)), static_cast<float>(static_cast<int8_t>(two >> 8)));
+        }
+        return __builtin_bit_cast(bf16x8, v);
+    } else {
+        u32x4 v, u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i])));
+            const float b = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
+            v[i] = upper_halves(a, b);
+            u[i] = upper_halves(without(a, 0xFFFF0000u), without(b, 0xFFFF0000u));
+        }
+        rest = __builtin_bit_cast(bf16x8, u);
+        return __builtin_bit_cast(bf16x8, v);
+    }
+}
+
+// What a wave streams: 16 weight rows x 128 bytes a step, the step's activations of up to 64 NB pieces, FP8 scales.
+template <int KIND, int X, int NB>
+struct Ring {
+    using R = Rows<KIND, X>;
+    static constexpr bool F8 = KIND == VBM_TYPE_F8_E4M3;
+    static constexpr int LOADS = 2 + NB + (F8 ? 1 : 0), STEP = 2048 + NB * 1024 + (F8 ? 256 : 0), NJ = R::VALUES / 32;
+
+    // Places of the two loads' 16-byte pieces as in the grouped products' rings: piece p of row r at place p ^ (r / 2 % 8) of
+    // its 128 bytes. Activations: entry c's pieces behind each other, p at place p ^ (c % 8), so that the lanes' reads
+    // of one piece of several entries spread over the banks.
+    // weights: eight rows from each base, offset: this lane's row there; rows, piece: the entry's row and the piece of each load of activations;
+    // scale: those of the lane's four rows of outputs. kb: the step.
+    static __device__ __forceinline__ void load(uint32_t at, const uint8_t * base0, const uint8_t * base1, const uint32_t (&offset)[2], const uint8_t * const (&rows)[NB],
+                                                const int (&piece)[NB], const float * scale, int kb, int k_bytes, int row_bytes) {
+        const int lane = threadIdx.x & 63, even = (lane & 7) ^ (lane >> 4), odd = even ^ 4;
+        const int64_t off = static_cast<int64_t>(kb) * 128;
+        // (a piece past the row's end reads the step's first one: zeros take its place in the registers)
+        const int e = kb * 128 + even * 16 < k_bytes ? even * 16 : 0, o = kb * 128 + odd * 16 < k_bytes ? odd * 16 : 0;
+        load_to_lds_16(base0 + off, offset[0] + e, at);
+        load_to_lds_16(base1 + off, offset[1] + o, at + 1024);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int b = kb * R::BYTES + piece[i] * 16;
+            load_to_lds_16(rows[i] + (b < row_bytes ? b : kb * R::BYTES), at + 2048 + i * 1024);
+        }
+        if constexpr (F8) load_to_lds_4(scale + kb, at + 2048 + NB * 1024);
+    }
+
+    // The step in `stage` added to acc: lane (q, r) has rows 4q .. 4q + 3 of column r. entry, term: this lane's column; left: bytes of a weight row from
+    // this lane's 32 bytes on.
+    static __device__ __forceinline__ f32x4 multiply(const uint8_t * stage, int entry, int term, int left, f32x4 acc) {
+        const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+        unsigned w[8];
+        *reinterpret_cast<u32x4 *>(w) = *reinterpret_cast<const u32x4 *>(stage + r * 128 + ((2 * q) ^ (r >> 1)) * 16);
+        *reinterpret_cast<u32x4 *>(w + 4) = *reinterpret_cast<const u32x4 *>(stage + r * 128 + ((2 * q + 1) ^ (r >> 1)) * 16);
+        const uint8_t * row = stage + 2048 + entry * R::BYTES;
+        auto piece = [&](int p) { return *reinterpret_cast<const u32x4 *>(row + (p ^ (entry & 7)) * 16); };
+        f32x4 sum = F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc;
+        const unsigned mask0 = term >= 1 ? 0xFFFF0000u : 0u, mask1 = term == 2 ? 0xFFFF0000u : 0u;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            u32x4 b;
+            if constexpr (X == VBM_TYPE_BF16) {
+                b = piece(q * NJ + j);
+            } else if constexpr (X == kTerms) {
+                b = piece(term * (R::VALUES / 8) + q * NJ + j);
+            } else {
+                float v[8];
+                if constexpr (X == VBM_TYPE_F32) {
+                    const f32x4 lo = __builtin_bit_cast(f32x4, piece((q * NJ + j) * 2)), hi = __builtin_bit_cast(f32x4, piece((q * NJ + j) * 2 + 1));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+                } else {
+                    const u32x4 h = piece(q * NJ + j);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h[i >> 1] >> (16 * (i & 1)))));
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    v[i] = without(v[i], mask0);
+                    if constexpr (X == VBM_TYPE_F32) v[i] = without(v[i], mask1);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = upper_halves(v[2 * i], v[2 * i + 1]);
+            }
+            unsigned a[4] = {w[one_byte(KIND) ? 2 * j : 4 * (j & 1)], w[one_byte(KIND) ? 2 * j + 1 : 4 * (j & 1) + 1],
+                             w[one_byte(KIND) ? 0 : 4 * (j & 1) + 2], w[one_byte(KIND) ? 0 : 4 * (j & 1) + 3]};
+            if (left < 32 && left <= (j * 2 / NJ) * 16) {    // (k ends at a multiple of 16 bytes)
+                b = u32x4{0, 0, 0, 0};
+                a[0] = a[1] = a[2] = a[3] = 0;
+            }
+            bf16x8 rest;
+            const bf16x8 x = __builtin_bit_cast(bf16x8, b), v = widened<KIND>(a, rest);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, x, sum, 0, 0, 0);
+            if constexpr (KIND == VBM_TYPE_F16) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rest, x, sum, 0, 0, 0);
+        }
+        if constexpr (F8) {
+            const float f = *reinterpret_cast<const float *>(stage + 2048 + NB * 1024 + lane * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(sum[i], f, acc[i]);
+            return acc;
+        }
+        return sum;
+    }
+};
+
+// ------------------------------------------------------------------------------------ gate and up
+// A row tile is 8 gate rows and the 8 up rows of the same values of h. SHARE waves share a tile's depth and join their sums through LDS; or
+// (SHARE 1) each wave takes `tiles` of its own, one after the other through its ring, without barriers.
+template <int KIND, int X, int NB, int SHARE>
+__global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
+    using S = Ring<KIND, X, NB>;
+    using R = Rows<KIND, X>;
+    constexpr int W = 4, D = 4, MOST_TILES = SHARE == 1 ? 8 : 1, TILES = W / SHARE * MOST_TILES;
+    constexpr bool kScaled = KIND == VBM_TYPE_I8;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[W * D * S::STEP];
+    __shared__ __attribute__((aligned(16))) float sums[W][16 * 16];                       // [column][row] of a wave's tile
+    __shared__ float row_bias[TILES * 16], row_scale[kScaled ? TILES * 16 : 1];
+    __shared__ int32_t ids[kMostEntries];
+    __shared__ int list[W][8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int q = lane >> 4, r = lane & 15;
+    route<W>(A, ids, blockIdx.x == 0);
+    __syncthreads();
+    const int index = static_cast<int>(blockIdx.x) / A.row_units, unit = static_cast<int>(blockIdx.x) - index * A.row_units;
+    int expert;
+    const int n = Slots(ids, A.entries, A.n_expert, A.capacity).find(index, A.capacity, expert, list[wave]);
+    if (!n) return;                                          // (the whole workgroup)
+    expert = __builtin_amdgcn_readfirstlane(expert);
+
+    const int row_tiles = A.inter >> 3, group = wave / SHARE;
+    const int first_tile = (unit * A.tiles * (W / SHARE)) + group, step_tiles = W / SHARE;   // this wave's: first_tile + step_tiles i
+    const int my_tiles = first_tile >= row_tiles ? 0 : std::min((row_tiles - first_tile + step_tiles - 1) / step_tiles, A.tiles);
+    const int k_begin = A.kb * (wave % SHARE) / SHARE, k_end = A.kb * (wave % SHARE + 1) / SHARE;
+    const uint8_t * weights = A.w + static_cast<int64_t>(expert) * A.rows * A.k_bytes;
+    uint8_t * mine = ring + wave * (D * S::STEP);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(mine));
+
+    // entries: the ones that this lane loads pieces of, and its column's
+    const int row_bytes = R::TERMS == 3 ? A.k_bytes / (one_byte(KIND) ? 1 : 2) * 4 : A.k_bytes / (one_byte(KIND) ? 1 : 2) * 2;
+    const uint8_t * rows[NB];
+    int piece[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int flat = 64 * i + lane, c = flat / R::PIECES, entry = list[wave][c < n ? c : 0];
+        rows[i] = static_cast<const uint8_t *>(A.x) + static_cast<int64_t>(entry / A.top_k) * row_bytes;
+        piece[i] = (flat % R::PIECES) ^ (c & 7);
+    }
+    const int column = r / R::TERMS < n ? r / R::TERMS : 0, term = r % R::TERMS;
+
+    int tile_next = 0, kb_next = k_begin, slot_next = 0;
+    const uint8_t * base = nullptr;
+    const uint32_t offset[2] = {static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(A.k_bytes), static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(A.k_bytes)};
+    const float * scale = nullptr;
+    auto enter = [&](int i) __attribute__((always_inline)) {
+        const int i0 = (first_tile + step_tiles * i) * 8;
+        base = weights + static_cast<int64_t>(i0) * A.k_bytes;
+        if constexpr (S::F8) scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + ((i0 + (q >= 2 ? A.inter : 0)) >> 7)) * A.kb;
+    };
+    auto issue = [&]() __attribute__((always_inline)) {
+        S::load(lds0 + slot_next * S::STEP, base, base + static_cast<int64_t>(A.inter) * A.k_bytes, offset, rows, piece, scale, kb_next, A.k_bytes, row_bytes);
+        slot_next = slot_next + 1 == D ? 0 : slot_next + 1;
+        if (kb_next + 1 < k_end) {
+            ++kb_next;
+        } else if (tile_next + 1 < my_tiles) {
+            kb_next = k_begin;
+            enter(++tile_next);
+        }
+    };
+    const bool streams = my_tiles > 0 && k_begin < k_end;
+    if (streams) {
+        enter(0);
+#pragma unroll
+        for (int i = 0; i < D; ++i) issue();
+    }
+    for (int i = threadIdx.x; i < step_tiles * A.tiles * 16; i += W * 64) {
+        const int at = (unit * A.tiles * step_tiles + (i >> 4)) * 8 + (i & 7) + (i & 8 ? A.inter : 0);
+        const bool live = (unit * A.tiles * step_tiles + (i >> 4)) < row_tiles;
+        row_bias[i] = A.bias && live ? A.bias[static_cast<int64_t>(expert) * A.rows + at] : 0.0f;
+        if constexpr (kScaled) row_scale[i] = live ? A.ws[static_cast<int64_t>(expert) * A.rows + at] : 0.0f;
+    }
+    __syncthreads();
+
+    // tile i's sums to h: lane (c, j) has value j of entry c
+    auto finish = [&](int i) __attribute__((always_inline)) {
+        const int c = lane >> 3, j = lane & 7, local = (group + step_tiles * i) * 16;
+        if (c >= n) return;
+        float gate = 0.0f, up = 0.0f;
+#pragma unroll
+        for (int s = 0; s < SHARE; ++s)
+#pragma unroll
+            for (int t = R::TERMS - 1; t >= 0; --t) {
+                gate += sums[wave + s][(c * R::TERMS + t) * 16 + j];
+                up += sums[wave + s][(c * R::TERMS + t) * 16 + 8 + j];
+            }
+        if constexpr (kScaled) gate *= row_scale[local + j], up *= row_scale[local + 8 + j];
+        const float v = glu_value(A.activation, gate + row_bias[local + j], up + row_bias[local + 8 + j], A.alpha, A.limit);
+        // its three terms
+        const float v1 = without(v, 0xFFFF0000u), v2 = without(v1, 0xFFFF0000u);
+        const int at = (first_tile + step_tiles * i) * 8 + j, kb = at / R::VALUES;
+        uint16_t * to = reinterpret_cast<uint16_t *>(A.h + (static_cast<int64_t>(list[wave][c]) * A.h_kb + kb) * A.h_step) + at % R::VALUES;
+        to[0] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v) >> 16);
+        to[R::VALUES] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v1) >> 16);
+        to[2 * R::VALUES] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v2) >> 16);
+    };
+
+    int slot = 0;
+    for (int i = 0; i < (SHARE == 1 ? my_tiles : 1); ++i) {
+        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+        if (streams) {
+            for (int kb = k_begin; kb < k_end; ++kb) {
+                landed<(D - 1) * S::LOADS>();
+                acc = S::multiply(mine + slot * S::STEP, column, term, A.k_bytes - kb * 128 - 32 * q, acc);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
+                issue();
+                slot = slot + 1 == D ? 0 : slot + 1;
+            }
+        }
+        *reinterpret_cast<f32x4 *>(&sums[wave][r * 16 + 4 * q]) = acc;
+        if constexpr (SHARE == 1) finish(i);
+    }
+    landed<0>();                                             // no load may land after the workgroup has ended
+    if constexpr (SHARE > 1) {
+        __syncthreads();
+        if (wave % SHARE == 0 && my_tiles > 0) finish(0);
+    }
+}
+
+// ------------------------------------------------------------------------------- down and combine
+// A workgroup takes 16 rows of the output for all slots; its waves share all their steps in contiguous runs, slot by slot. A wave's sums of a slot
+// go to the entries' places in LDS, except for a slot that an earlier wave began: those are added up behind it, in the waves' order.
+template <int KIND, int NB>
+__global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
+    using S = Ring<KIND, kTerms, NB>;
+    using R = Rows<KIND, kTerms>;
+    constexpr int W = 8, D = NB <= 2 ? 4 : 3;              // (what fits in LDS)
+    constexpr bool kScaled = KIND == VBM_TYPE_I8;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[W * D * S::STEP];
+    __shared__ __attribute__((aligned(16))) float y[kMostEntries * 16], heads[W][R::MOST * 16];
+    __shared__ int32_t ids[kMostEntries];
+    __shared__ int experts[kMostEntries], counts[kMostEntries], list[kMostEntries * R::MOST], head_slot[W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int q = lane >> 4, r = lane & 15, n0 = static_cast<int>(blockIdx.x) * 16;
+    for (int i = threadIdx.x; i < A.entries; i += W * 64) ids[i] = A.ids[i];
+    __syncthreads();
+    const Slots slots(ids, A.entries, A.n_expert, A.capacity);
+    const int n_slots = slots.count();
+    if (wave == 0) slots.table(A.capacity, experts, counts, list);
+    __syncthreads();
+
+    const int total = n_slots * A.kb, begin = static_cast<int>(static_cast<int64_t>(total) * wave / W), end = static_cast<int>(static_cast<int64_t>(total) * (wave + 1) / W);
+    uint8_t * mine = ring + wave * (D * S::STEP);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(mine));
+    const int row_bytes = A.kb * R::BYTES;
+
+    int next = begin, slot_next = A.kb ? begin / A.kb : 0, kb_next = begin - slot_next * A.kb, place_next = 0;
+    const uint8_t * base = nullptr, * rows[NB];
+    int piece[NB];
+    uint32_t offset[2];
+#pragma unroll
+    for (int l = 0; l < 2; ++l) {
+        const int n = n0 + 8 * l + (lane >> 3);
+        offset[l] = static_cast<uint32_t>((n < A.rows ? n : A.rows - 1) - n0) * static_cast<uint32_t>(A.k_bytes);
+    }
+    const float * scale = nullptr;
+    auto enter = [&](int s) __attribute__((always_inline)) {
+        const int expert = __builtin_amdgcn_readfirstlane(experts[s]), n = counts[s];
+        base = A.w + (static_cast<int64_t>(expert) * A.rows + n0) * A.k_bytes;
+        if constexpr (S::F8) scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + (n0 >> 7)) * A.kb;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int flat = 64 * i + lane, c = flat / R::PIECES, entry = list[s * A.capacity + (c < n ? c : 0)];
+            rows[i] = static_cast<const uint8_t *>(A.x) + static_cast<int64_t>(entry) * row_bytes;
+            piece[i] = (flat % R::PIECES) ^ (c & 7);
+        }
+    };
+    auto issue = [&]() __attribute__((always_inline)) {
+        S::load(lds0 + place_next * S::STEP, base, base, offset, rows, piece, scale, kb_next, A.k_bytes, row_bytes);
+        place_next = place_next + 1 == D ? 0 : place_next + 1;
+        if (next + 1 < end) {                                // (past the end the last step again, so that the waits' counts hold)
+            ++next;
+            if (++kb_next == A.kb) {
+                kb_next = 0;
+                enter(++slot_next);
+            }
+        }
+    };
+    if (lane == 0) head_slot[wave] = -1;
+    if (begin < end) {
+        int s = slot_next, kb = kb_next, place = 0;
+        enter(s);
+#pragma unroll
+        for (int i = 0; i < D; ++i) issue();
+        const int column = r / 3, term = r % 3;
+        bool head = kb > 0;
+        int n = counts[s];
+        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = begin; i < end; ++i) {
+            landed<(D - 1) * S::LOADS>();
+            acc = S::multiply(mine + place * S::STEP, column < n ? column : 0, term, A.k_bytes - kb * 128 - 32 * q, acc);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
+            issue();
+            place = place + 1 == D ? 0 : place + 1;
+            if (++kb == A.kb || i + 1 == end) {
+                // an entry's three columns are neighbouring lanes
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float sum = acc[e];                // (a bit cast of the vector's element itself would take the first one's)
+                    const int v = __builtin_bit_cast(int, sum);
+                    const float v1 = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, 0x101, 0xF, 0xF, true));
+                    const float v2 = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, 0x102, 0xF, 0xF, true));
+                    acc[e] += v2 + v1;
+                }
+                if (term == 0 && column < n) {
+                    float * to = head ? &heads[wave][column * 16] : y + list[s * A.capacity + column] * 16;
+                    *reinterpret_cast<f32x4 *>(to + 4 * q) = acc;
+                }
+                if (head && lane == 0) head_slot[wave] = s;
+                acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                head = false;
+                kb = 0;
+                if (i + 1 < end) n = counts[++s];
+            }
+        }
+        landed<0>();                                         // no load may land after the workgroup has ended
+    }
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < W; ++w) {
+            const int s = head_slot[w];
+            if (s < 0) continue;
+            for (int i = lane; i < counts[s] * 16; i += 64) y[list[s * A.capacity + (i >> 4)] * 16 + (i & 15)] += heads[w][i];
+        }
+    }
+    __syncthreads();
+    // output row n0 + i % 16 of token i / 16: the ranks in their order
+    for (int i = threadIdx.x; i < A.n_tokens * 16; i += W * 64) {
+        const int t = i >> 4, n = n0 + (i & 15);
+        if (n >= A.rows) continue;
+        float v = 0.0f;
+        for (int k = 0; k < A.top_k; ++k) {
+            const int entry = t * A.top_k + k, expert = ids[entry];
+            if (expert == -1) continue;
+            float e = __builtin_nanf("");
+            if (static_cast<unsigned>(expert) < static_cast<unsigned>(A.n_expert)) {
+                const int64_t at = static_cast<int64_t>(expert) * A.rows + n;
+                e = y[entry * 16 + (i & 15)];
+                if constexpr (kScaled) e *= A.ws[at];
+                if (A.bias) e += A.bias[at];
+            }
+            v += A.weights[entry] * e;
+        }
+        const int64_t at = static_cast<int64_t>(t) * A.rows + n;
+        if (A.out_type == VBM_TYPE_F32) static_cast<float *>(A.out)[at] = v;
+        else if (A.out_type == VBM_TYPE_BF16) static_cast<__bf16 *>(A.out)[at] = static_cast<__bf16>(v);
+        else static_cast<_Float16 *>(A.out)[at] = static_cast<_Float16>(v);
+    }
+}
+
+struct FewCall {
+    int kind, x_type;
+    FewArgs up, down;              // of the two launches
+    int64_t slots;                 // at most, and expected
+    double expected;
+    size_t h_at, bytes;            // of the workspace
+};
+
+int64_t align_256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Checks everything but the buffers of one call.
+FewCall few_call(const vbm_moe_few_desc * d, int64_t n_tokens) {
+    require(d != nullptr, "null description");
+    const vbm_weights & g = d->gate_up, & w = d->down;
+    const bool bytes = one_byte(g.type);
+    require(bytes || g.type == VBM_TYPE_F16 || g.type == VBM_TYPE_BF16, "weights must be I8, F8_E4M3, F16 or BF16");
+    require(w.type == g.type, "gate_up and down must be of one type");
+    require(g.n_groups > 0 && g.n_groups <= kMaxRouteExperts && w.n_groups == g.n_groups, "gate_up and down need the same number of experts, 1..1024");
+    require(g.k > 0 && g.k < (int64_t{1} << 23) && w.k > 0 && w.k < (int64_t{1} << 23), "rows and k out of range");
+    require(w.rows == g.k && g.rows == 2 * w.k, "gate_up must be [2 * I][H] and down [H][I]");
+    require(g.k % (bytes ? 16 : 8) == 0 && w.k % (bytes ? 16 : 8) == 0, bytes ? "H and I must be multiples of 16" : "H and I must be multiples of 8");
+    require(g.data && w.data && (!bytes || (g.scales && w.scales)), "null weights");
+    auto at = [](const void * p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+    require(at(g.data, 16) && at(w.data, 16), "weights must be 16-byte aligned");
+    require(at(g.scales, 4) && at(w.scales, 4) && at(g.bias, 4) && at(w.bias, 4), "buffers must be aligned to their types");
+    require(d->activation == VBM_ACT_SILU || d->activation == VBM_ACT_SWIGLU_OAI, "unknown activation");
+    require(d->top_k > 0 && d->top_k <= g.n_groups && d->top_k <= 64, "top_k must be 1..n_experts, at most 64");
+    require(n_tokens >= 0 && n_tokens <= kMostTokens && n_tokens * d->top_k <= kMostEntries, "at most 16 tokens and 128 (token, rank) pairs");
+
+    FewCall c{};
+    c.kind = g.type;
+    FewArgs & a = c.up;
+    a.w = static_cast<const uint8_t *>(g.data);
+    a.ws = g.scales;
+    a.bias = g.bias;
+    a.n_tokens = static_cast<int>(n_tokens);
+    a.top_k = static_cast<int>(d->top_k);
+    a.n_expert = static_cast<int>(g.n_groups);
+    a.entries = a.n_tokens * a.top_k;
+    a.inter = static_cast<int>(w.k);
+    a.activation = d->activation;
+    a.alpha = d->alpha;
+    a.limit = d->limit;
+    const int size = bytes ? 1 : 2;
+    a.rows = static_cast<int>(g.rows);
+    a.k_bytes = static_cast<int>(g.k) * size;
+    a.kb = (a.k_bytes + 127) / 128;
+    a.h_kb = (a.inter * size + 127) / 128;
+    a.h_step = bytes ? Rows<VBM_TYPE_I8, kTerms>::BYTES : Rows<VBM_TYPE_BF16, kTerms>::BYTES;
+    FewArgs & b = c.down;
+    b = a;
+    b.w = static_cast<const uint8_t *>(w.data);
+    b.ws = w.scales;
+    b.bias = w.bias;
+    b.rows = static_cast<int>(w.rows);
+    b.k_bytes = a.inter * size;
+    b.kb = a.h_kb;
+    // experts that are hit if every token takes top_k of them at random
+    double missed = 1.0;
+    for (int64_t t = 0; t < n_tokens; ++t) missed *= 1.0 - static_cast<double>(a.top_k) / a.n_expert;
+    c.expected = std::max(1.0, a.n_expert * (1.0 - missed));
+    c.slots = a.entries;
+    c.h_at = static_cast<size_t>(2 * align_256(4 * kMostEntries));
+    c.bytes = c.h_at + static_cast<size_t>(a.entries) * a.h_kb * a.h_step;
+    return c;
+}
+
+// Shared depth for few tiles: four waves a tile until each of the 1024 that run at once has four of its own.
+template <int KIND, int X>
+void launch_gate_up(const FewCall & c, hipStream_t stream) {
+    using R = Rows<KIND, X>;
+    FewArgs a = c.up;
+    a.capacity = std::min(R::MOST, a.n_tokens);
+    const int64_t row_tiles = a.inter / 8;
+    const double tiles = c.expected * static_cast<double>(row_tiles);
+    auto go = [&](auto nb_c, auto share_c) {
+        constexpr int NB = decltype(nb_c)::value, SHARE = decltype(share_c)::value, AT_ONCE = 4 / SHARE;
+        a.tiles = SHARE == 1 ? static_cast<int>(std::max(1.0, std::min(8.0, tiles / 4096))) : 1;
+        a.row_units = static_cast<int>((row_tiles + AT_ONCE * a.tiles - 1) / (AT_ONCE * a.tiles));
+        const int64_t blocks = c.slots * a.row_units;
+        require(blocks < (int64_t{1} << 24), "too many outputs for one launch");
+        hipLaunchKernelGGL((few_gate_up_kernel<KIND, X, NB, SHARE>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+        check_hip(hipGetLastError(), "few tokens gate_up launch");
+    };
+    auto shape = [&](auto nb_c) {
+        if (tiles >= 4096) go(nb_c, std::integral_constant<int, 1>{});
+        else go(nb_c, std::integral_constant<int, 4>{});
+    };
+    const int nb = R::loads(a.capacity);
+    if (nb == 1) return shape(std::integral_constant<int, 1>{});
+    if constexpr (R::loads(R::MOST) >= 2) {
+        if (nb == 2) return shape(std::integral_constant<int, 2>{});
+    }
+    if constexpr (R::loads(R::MOST) >= 3) shape(std::integral_constant<int, 3>{});
+}
+
+template <int KIND>
+void launch_down(const FewCall & c, hipStream_t stream) {
+    using R = Rows<KIND, kTerms>;
+    FewArgs b = c.down;
+    b.capacity = std::min(R::MOST, b.n_tokens);
+    auto go = [&](auto nb_c) {
+        hipLaunchKernelGGL((few_down_kernel<KIND, decltype(nb_c)::value>), dim3(static_cast<unsigned>((b.rows + 15) / 16)), dim3(512), 0, stream, b);
+        check_hip(hipGetLastError(), "few tokens down launch");
+    };
+    const int nb = R::loads(b.capacity);
+    if (nb == 1) return go(std::integral_constant<int, 1>{});
+    if (nb == 2) return go(std::integral_constant<int, 2>{});
+    if constexpr (R::loads(R::MOST) >= 3) go(std::integral_constant<int, 3>{});
+}
+
+template <int KIND>
+void launch_few(const FewCall & c, hipStream_t stream) {
+    if (c.x_type == VBM_TYPE_F32) launch_gate_up<KIND, VBM_TYPE_F32>(c, stream);
+    else if (c.x_type == VBM_TYPE_F16) launch_gate_up<KIND, VBM_TYPE_F16>(c, stream);
+    else launch_gate_up<KIND, VBM_TYPE_BF16>(c, stream);
+    launch_down<KIND>(c, stream);
+}
+
+}  // namespace
+}  // namespace vbm
+
+using namespace vbm;
+
+extern "C" {
+
+vbm_status vbm_moe_few_workspace(const vbm_moe_few_desc * desc, int64_t n_tokens, size_t * bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "null bytes");
+        *bytes = few_call(desc, n_tokens).bytes;
+    });
+}
+
+vbm_status vbm_moe_few_forward(const vbm_moe_few_desc * desc, int x_type, const void * x, const float * logits, int32_t * ids, float * weights,
+                               int64_t n_tokens, int out_type, void * out, void * workspace, size_t workspace_bytes, void * stream) {
+    return guarded([&] {
+        FewCall c = few_call(desc, n_tokens);
+        auto type = [](int t) { return t == VBM_TYPE_F32 || t == VBM_TYPE_F16 || t == VBM_TYPE_BF16; };
+        require(type(x_type), "x must be F32, F16 or BF16");
+        require(type(out_type), "out must be F32, F16 or BF16");
+        if (n_tokens == 0) return;
+        auto at = [](const void * p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+        require(x && out && workspace, "null buffer");
+        require(logits || (ids && weights), "neither logits nor ids and weights");
+        require(at(x, 16) && at(workspace, 16), "x and workspace must be 16-byte aligned");
+        require(at(out, out_type == VBM_TYPE_F32 ? 4 : 2) && at(logits, 4) && at(ids, 4) && at(weights, 4), "buffers must be aligned to their types");
+        require(workspace_bytes >= c.bytes, "workspace too small");
+        uint8_t * space = static_cast<uint8_t *>(workspace);
+        int32_t * chosen = ids ? ids : reinterpret_cast<int32_t *>(space);
+        float * shares = weights ? weights : reinterpret_cast<float *>(space + align_256(4 * kMostEntries));
+        c.x_type = x_type;
+        c.up.x = x;
+        c.up.logits = logits;
+        c.up.ids = c.down.ids = chosen;
+        c.up.ids_out = chosen;
+        c.up.weights_out = shares;
+        c.up.h = space + c.h_at;
+        c.down.x = space + c.h_at;
+        c.down.weights = shares;
+        c.down.out = out;
+        c.down.out_type = out_type;
+        if (c.kind == VBM_TYPE_F8_E4M3) launch_few<VBM_TYPE_F8_E4M3>(c, as_stream(stream));
+        else if (c.kind == VBM_TYPE_I8) launch_few<VBM_TYPE_I8>(c, as_stream(stream));
+        else if (c.kind == VBM_TYPE_F16) launch_few<VBM_TYPE_F16>(c, as_stream(stream));
+        else launch_few<VBM_TYPE_BF16>(c, as_stream(stream));
+    });
+}
+
+}  // extern "C"

@@ -123,6 +123,11 @@ class Weights(C.Structure):
     _fields_ = [("type", C.c_int), ("data", vp), ("scales", vp), ("bias", vp), ("n_groups", i64), ("rows", i64), ("k", i64)]
 
 
+class MoeFewDesc(C.Structure):
+    """vbm_moe_few_desc: the experts of a layer for a few tokens, as vbm_weights."""
+    _fields_ = [("gate_up", Weights), ("down", Weights), ("top_k", i64), ("activation", C.c_int), ("alpha", C.c_float), ("limit", C.c_float)]
+
+
 # name -> argtypes (all return vbm_status as c_int)
 SIGNATURES = {
     "vbm_device_count": [C.POINTER(C.c_int)],
@@ -179,6 +184,8 @@ SIGNATURES = {
     "vbm_mul_mat_i8": [C.POINTER(Weights), vp, vp, i64, C.c_int, vp, vp],
     "vbm_mul_mat_fp8": [C.POINTER(Weights), vp, vp, i64, C.c_int, vp, vp],
     "vbm_grouped_mul_mat": [C.POINTER(Weights), vp, vp, i64, vp, i64, vp, i64, vp, i64, C.c_int, vp, vp],
+    "vbm_moe_few_workspace": [C.POINTER(MoeFewDesc), i64, C.POINTER(sz)],
+    "vbm_moe_few_forward": [C.POINTER(MoeFewDesc), C.c_int, vp, vp, vp, vp, i64, C.c_int, vp, vp, sz, vp],
     "vbm_moe_layer_workspace": [C.POINTER(MoeLayerDesc), i64, C.POINTER(sz)],
     "vbm_moe_layer_forward": [C.POINTER(MoeLayerDesc), vp, vp, i64, vp, vp, vp, vp, sz, vp],
     "vbm_moe_layer_forward_profiled": [C.POINTER(MoeLayerDesc), vp, vp, i64, vp, vp, vp, vp, sz, vp, vp],
