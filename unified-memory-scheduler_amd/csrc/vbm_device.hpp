@@ -118,45 +118,6 @@ __device__ __forceinline__ float half_wave_max(float v) {
     return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F)));
 }
 
-// One wavefront's top-k over n <= 64 NPL routing keys held in registers (lg[i]: expert lane + 64 i,
-// already route_key'd, so never NaN), in the total order (value desc, then lower index;
-// tools/trace/topk-tie-probe.cpp:111-113): pick j is the best element strictly after pick j - 1.
-// Each round takes the wave maximum of the lanes' best remaining candidates (DPP and a swizzle,
-// no LDS traffic), then the lowest expert index holding it with one ballot per register row.
-// Lane j < k returns pick j in (sel_v, sel_i). No barrier: every wave can route for itself.
-template <int NPL>
-__device__ __forceinline__ void wave_topk_regs(const float (&lg)[NPL], int n, int k, float & sel_v, int & sel_i) {
-    const int lane = threadIdx.x & 63;
-    float prev_v = INFINITY;
-    int prev_i = -1;
-    sel_v = 0.0f;
-    sel_i = -1;
-    for (int j = 0; j < k; ++j) {
-        float best = -INFINITY;
-        int best_i = -1;
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-            const int c = lane + 64 * i;
-            const float v = lg[i];
-            const bool after_prev = v < prev_v || (v == prev_v && c > prev_i);
-            if (c < n && after_prev && (best_i < 0 || v > best)) { best = v; best_i = c; }
-        }
-        const float h = half_wave_max(best);
-        const float m0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, h), 0));
-        const float m1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, h), 32));
-        const float top = m0 > m1 ? m0 : m1;
-        int pick = -1;
-#pragma unroll
-        for (int i = NPL - 1; i >= 0; --i) {
-            const uint64_t m = __ballot(best_i >= 0 && best == top && (best_i >> 6) == i);
-            if (m) pick = 64 * i + __builtin_ctzll(m);
-        }
-        if (lane == j) { sel_v = top; sel_i = pick; }
-        prev_v = top;
-        prev_i = pick;
-    }
-}
-
 // ggml soft_max over the k picks held by lanes 0..k-1 (expf(v - max), sum in double in pick order,
 // scale by (float)(1/sum)); returns the weight of pick `lane` (lane < k).
 __device__ __forceinline__ float wave_pick_softmax(float sel_v, int k) {

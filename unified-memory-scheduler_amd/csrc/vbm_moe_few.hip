@@ -18,6 +18,7 @@
 // The weights stream as in the grouped products: 16 rows by 128 bytes a step, loaded straight to a ring in LDS of each wave, with the
 // activations of the step behind them (they come from the L2, and the waits count all loads alike).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "vbm_device.hpp"
@@ -33,7 +34,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kMostTokens = 16, kMostEntries = 128;
+constexpr int kMostTokens = 16, kMostEntries = 128, kMostTiles = 4;   // (tiles of a wave)
 constexpr int kTerms = -1;                     // the type of h: three bf16 terms of each value, a step's first, second, third
 
 constexpr bool one_byte(int kind) { return kind == VBM_TYPE_F8_E4M3 || kind == VBM_TYPE_I8; }
@@ -151,6 +152,53 @@ struct Slots {
     }
 };
 
+// Maximum over the wave, the same in all lanes.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+        v = o > v ? o : v;
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});   // row_shr 1, 2, 4, 8
+    step(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    step(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    step(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});   // row 0's last to row 1, row 2's to row 3
+    step(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});   // lane 31's to the upper half
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+// One wave's top-k of n <= 64 NPL logits, lg[c]: that of expert lane + 64 c, in the router's order (value desc, then lower index, NaN as -inf):
+// lane j < k gets pick j. The keys are the values' bits, which order as they do once the sign is taken care of; 0 is none left. A round is
+// a maximum over lanes in registers (with an exchange through LDS in it, as the router's has, a token took about 1 us more).
+template <int NPL>
+__device__ __forceinline__ void top_k(const float (&lg)[NPL], int n, int k, float & value, int & id) {
+    const int lane = threadIdx.x & 63;
+    uint32_t key[NPL];
+#pragma unroll
+    for (int c = 0; c < NPL; ++c) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, route_key(lg[c]) + 0.0f);   // (-0 as 0)
+        key[c] = lane + 64 * c < n ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
+    }
+    uint32_t mine = 0;
+    id = -1;
+    for (int j = 0; j < k; ++j) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int c = 1; c < NPL; ++c) best = key[c] > best ? key[c] : best;
+        const uint32_t top = wave_max(best);
+        int pick = -1;
+#pragma unroll
+        for (int c = NPL - 1; c >= 0; --c) {
+            const uint64_t m = __ballot(key[c] == top);
+            if (m) pick = 64 * c + __builtin_ctzll(m);
+        }
+#pragma unroll
+        for (int c = 0; c < NPL; ++c) key[c] = pick == lane + 64 * c ? 0u : key[c];
+        if (lane == j) mine = top, id = pick;
+    }
+    value = __builtin_bit_cast(float, mine & 0x80000000u ? mine & 0x7FFFFFFFu : ~mine);
+}
+
 // ids (and weights) of the tokens into LDS, by top-k of the logits or from the caller; W waves.
 template <int W>
 __device__ __forceinline__ void route(const FewArgs & A, int32_t * ids, bool writes) {
@@ -165,8 +213,8 @@ __device__ __forceinline__ void route(const FewArgs & A, int32_t * ids, bool wri
             float lg[NPL], value;
             int id;
 #pragma unroll
-            for (int c = 0; c < NPL; ++c) lg[c] = lane + 64 * c < A.n_expert ? route_key(A.logits[static_cast<int64_t>(t) * A.n_expert + lane + 64 * c]) : 0.0f;
-            wave_topk_regs<NPL>(lg, A.n_expert, A.top_k, value, id);
+            for (int c = 0; c < NPL; ++c) lg[c] = lane + 64 * c < A.n_expert ? A.logits[static_cast<int64_t>(t) * A.n_expert + lane + 64 * c] : 0.0f;
+            top_k<NPL>(lg, A.n_expert, A.top_k, value, id);
             if (lane < A.top_k) ids[t * A.top_k + lane] = id;
             if (writes) {
                 const float w = wave_pick_softmax(value, A.top_k);
@@ -220,44 +268,88 @@ __device__ __forceinline__ bf16x8 widened(const unsigned * w, bf16x8 & rest) {
     }
 }
 
-// What a wave streams: 16 weight rows x 128 bytes a step, the step's activations of up to 64 NB pieces, FP8 scales.
-template <int KIND, int X, int NB>
+// The same in all lanes, which the compiler does not see everywhere.
+__device__ __forceinline__ const uint8_t * uniform(const uint8_t * p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+    return reinterpret_cast<const uint8_t *>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// What a wave streams: G times 16 weight rows x 128 bytes a step, the step's activations of up to 64 NB pieces, FP8 scales.
+template <int KIND, int X, int NB, int G>
 struct Ring {
     using R = Rows<KIND, X>;
     static constexpr bool F8 = KIND == VBM_TYPE_F8_E4M3;
-    static constexpr int LOADS = 2 + NB + (F8 ? 1 : 0), STEP = 2048 + NB * 1024 + (F8 ? 256 : 0), NJ = R::VALUES / 32;
+    // (LOADS: a step's at least. The waits count on these; a step with more entries has more of them, and then somewhat more than the
+    // oldest step is waited for. Loads for nobody instead, by one lane, took 10 ns a step of a CU, of 70.)
+    static constexpr int LOADS = 2 * G + 1 + (F8 ? 1 : 0), ACTIVATIONS = G * 2048, SCALES = ACTIVATIONS + NB * 1024, STEP = SCALES + (F8 ? 256 : 0);
+    static constexpr int NJ = R::VALUES / 32;
 
-    // Places of the two loads' 16-byte pieces as in the grouped products' rings: piece p of row r at place p ^ (r / 2 % 8) of
+    // What the lane loads: its rows of weights (offset from the groups' bases), the entry's row and the piece of each load of activations; `live` loads
+    // are for the slot's entries.
+    struct Source {
+        const uint8_t * base[G];
+        uint32_t offset[2 * G];
+        const uint8_t * rows[NB];
+        int piece[NB], live;
+        const float * scale;
+    };
+    // list: the n entries of the slot; row_of(entry): its activations.
+    template <class F>
+    static __device__ __forceinline__ void enter(Source & s, const int * list, int n, const F & row_of) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int flat = 64 * i + lane, c = flat / R::PIECES;
+            s.rows[i] = row_of(list[c < n ? c : 0]);
+            s.piece[i] = (flat % R::PIECES) ^ (c & 7);
+        }
+        s.live = __builtin_amdgcn_readfirstlane(R::loads(n));
+    }
+
+    // Places of the weights' 16-byte pieces as in the grouped products' rings: piece p of row r at place p ^ (r / 2 % 8) of
     // its 128 bytes. Activations: entry c's pieces behind each other, p at place p ^ (c % 8), so that the lanes' reads
     // of one piece of several entries spread over the banks.
-    // weights: eight rows from each base, offset: this lane's row there; rows, piece: the entry's row and the piece of each load of activations;
-    // scale: those of the lane's four rows of outputs. kb: the step.
-    static __device__ __forceinline__ void load(uint32_t at, const uint8_t * base0, const uint8_t * base1, const uint32_t (&offset)[2], const uint8_t * const (&rows)[NB],
-                                                const int (&piece)[NB], const float * scale, int kb, int k_bytes, int row_bytes) {
+    static __device__ __forceinline__ void load(uint32_t at, const Source & s, int kb, int k_bytes, int row_bytes) {
         const int lane = threadIdx.x & 63, even = (lane & 7) ^ (lane >> 4), odd = even ^ 4;
         const int64_t off = static_cast<int64_t>(kb) * 128;
         // (a piece past the row's end reads the step's first one: zeros take its place in the registers)
         const int e = kb * 128 + even * 16 < k_bytes ? even * 16 : 0, o = kb * 128 + odd * 16 < k_bytes ? odd * 16 : 0;
-        load_to_lds_16(base0 + off, offset[0] + e, at);
-        load_to_lds_16(base1 + off, offset[1] + o, at + 1024);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const uint8_t * base = uniform(s.base[g] + off);
+            load_to_lds_16(base, s.offset[2 * g] + e, at + g * 2048);
+            load_to_lds_16(base, s.offset[2 * g + 1] + o, at + g * 2048 + 1024);
+        }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int b = kb * R::BYTES + piece[i] * 16;
-            load_to_lds_16(rows[i] + (b < row_bytes ? b : kb * R::BYTES), at + 2048 + i * 1024);
+            if (i && i >= s.live) break;
+            const int b = kb * R::BYTES + s.piece[i] * 16;
+            load_to_lds_16(s.rows[i] + (b < row_bytes ? b : kb * R::BYTES), at + ACTIVATIONS + i * 1024);
         }
-        if constexpr (F8) load_to_lds_4(scale + kb, at + 2048 + NB * 1024);
+        if constexpr (F8) load_to_lds_4(s.scale + kb, at + SCALES);
     }
 
-    // The step in `stage` added to acc: lane (q, r) has rows 4q .. 4q + 3 of column r. entry, term: this lane's column; left: bytes of a weight row from
-    // this lane's 32 bytes on.
-    static __device__ __forceinline__ f32x4 multiply(const uint8_t * stage, int entry, int term, int left, f32x4 acc) {
+    // The step in `stage` added to acc: lane (q, r) has rows 4q .. 4q + 3 of column r of each group. entry, term: this lane's column.
+    static __device__ __forceinline__ void multiply(const uint8_t * stage, int entry, int term, int kb, int k_bytes, f32x4 (&acc)[G]) {
+        if ((kb + 1) * 128 <= k_bytes) multiply_step<false>(stage, entry, term, 128, acc);
+        else multiply_step<true>(stage, entry, term, k_bytes - kb * 128 - 32 * static_cast<int>(threadIdx.x >> 4 & 3), acc);
+    }
+    // TAIL: the row's last step is not a whole one; `left` bytes of it are from this lane's 32 on.
+    template <bool TAIL>
+    static __device__ __forceinline__ void multiply_step(const uint8_t * stage, int entry, int term, int left, f32x4 (&acc)[G]) {
         const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
-        unsigned w[8];
-        *reinterpret_cast<u32x4 *>(w) = *reinterpret_cast<const u32x4 *>(stage + r * 128 + ((2 * q) ^ (r >> 1)) * 16);
-        *reinterpret_cast<u32x4 *>(w + 4) = *reinterpret_cast<const u32x4 *>(stage + r * 128 + ((2 * q + 1) ^ (r >> 1)) * 16);
-        const uint8_t * row = stage + 2048 + entry * R::BYTES;
+        unsigned w[G][8];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            *reinterpret_cast<u32x4 *>(w[g]) = *reinterpret_cast<const u32x4 *>(stage + g * 2048 + r * 128 + ((2 * q) ^ (r >> 1)) * 16);
+            *reinterpret_cast<u32x4 *>(w[g] + 4) = *reinterpret_cast<const u32x4 *>(stage + g * 2048 + r * 128 + ((2 * q + 1) ^ (r >> 1)) * 16);
+        }
+        const uint8_t * row = stage + ACTIVATIONS + entry * R::BYTES;
         auto piece = [&](int p) { return *reinterpret_cast<const u32x4 *>(row + (p ^ (entry & 7)) * 16); };
-        f32x4 sum = F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc;
+        f32x4 sum[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) sum[g] = F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[g];
         const unsigned mask0 = term >= 1 ? 0xFFFF0000u : 0u, mask1 = term == 2 ? 0xFFFF0000u : 0u;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -285,39 +377,60 @@ struct Ring {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) b[i] = upper_halves(v[2 * i], v[2 * i + 1]);
             }
-            unsigned a[4] = {w[one_byte(KIND) ? 2 * j : 4 * (j & 1)], w[one_byte(KIND) ? 2 * j + 1 : 4 * (j & 1) + 1],
-                             w[one_byte(KIND) ? 0 : 4 * (j & 1) + 2], w[one_byte(KIND) ? 0 : 4 * (j & 1) + 3]};
-            if (left < 32 && left <= (j * 2 / NJ) * 16) {    // (k ends at a multiple of 16 bytes)
-                b = u32x4{0, 0, 0, 0};
-                a[0] = a[1] = a[2] = a[3] = 0;
-            }
-            bf16x8 rest;
-            const bf16x8 x = __builtin_bit_cast(bf16x8, b), v = widened<KIND>(a, rest);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, x, sum, 0, 0, 0);
-            if constexpr (KIND == VBM_TYPE_F16) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rest, x, sum, 0, 0, 0);
-        }
-        if constexpr (F8) {
-            const float f = *reinterpret_cast<const float *>(stage + 2048 + NB * 1024 + lane * 4);
+            const bool past = TAIL && left <= (j * 2 / NJ) * 16;   // (k ends at a multiple of 16 bytes)
+            if (past) b = u32x4{0, 0, 0, 0};
+            const bf16x8 x = __builtin_bit_cast(bf16x8, b);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(sum[i], f, acc[i]);
-            return acc;
+            for (int g = 0; g < G; ++g) {
+                constexpr int N = one_byte(KIND) ? 2 : 4;        // words of eight weights
+                unsigned a[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) a[i] = past ? 0u : w[g][N * j + i];
+                bf16x8 rest;
+                const bf16x8 v = widened<KIND>(a, rest);
+                sum[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, x, sum[g], 0, 0, 0);
+                if constexpr (KIND == VBM_TYPE_F16) sum[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rest, x, sum[g], 0, 0, 0);
+            }
         }
-        return sum;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if constexpr (F8) {
+                const float f = *reinterpret_cast<const float *>(stage + SCALES + g * (256 / G));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[g][i] = __builtin_fmaf(sum[g][i], f, acc[g][i]);
+            } else {
+                acc[g] = sum[g];
+            }
+        }
     }
 };
 
+// Lane (q, r) with an entry's first column: its terms' columns, which are the neighbouring lanes, added up.
+template <int TERMS>
+__device__ __forceinline__ f32x4 over_terms(f32x4 acc) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float sum = acc[e];                            // (a bit cast of the vector's element itself would take the first one's)
+        const int v = __builtin_bit_cast(int, sum);
+        float rest = 0.0f;
+        if constexpr (TERMS > 2) rest = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, 0x102, 0xF, 0xF, true));
+        if constexpr (TERMS > 1) rest += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, 0x101, 0xF, 0xF, true));
+        acc[e] = sum + rest;
+    }
+    return acc;
+}
+
 // ------------------------------------------------------------------------------------ gate and up
-// A row tile is 8 gate rows and the 8 up rows of the same values of h. SHARE waves share a tile's depth and join their sums through LDS; or
+// A row tile is 16 gate rows and the 16 up rows of the same values of h. SHARE waves share a tile's depth and join their sums through LDS; or
 // (SHARE 1) each wave takes `tiles` of its own, one after the other through its ring, without barriers.
 template <int KIND, int X, int NB, int SHARE>
 __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
-    using S = Ring<KIND, X, NB>;
+    using S = Ring<KIND, X, NB, 2>;
     using R = Rows<KIND, X>;
-    constexpr int W = 4, D = 4, MOST_TILES = SHARE == 1 ? 8 : 1, TILES = W / SHARE * MOST_TILES;
+    constexpr int W = 4, D = NB <= 2 ? 3 : 2, MOST_TILES = SHARE == 1 ? kMostTiles : 1, TILES = W / SHARE * MOST_TILES;   // (two workgroups a CU)
     constexpr bool kScaled = KIND == VBM_TYPE_I8;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[W * D * S::STEP];
-    __shared__ __attribute__((aligned(16))) float sums[W][16 * 16];                       // [column][row] of a wave's tile
-    __shared__ float row_bias[TILES * 16], row_scale[kScaled ? TILES * 16 : 1];
+    __shared__ __attribute__((aligned(16))) float row_bias[TILES * 32], row_scale[kScaled ? TILES * 32 : 4];   // [tile][gate, up][16]
     __shared__ int32_t ids[kMostEntries];
     __shared__ int list[W][8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -330,39 +443,36 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
     if (!n) return;                                          // (the whole workgroup)
     expert = __builtin_amdgcn_readfirstlane(expert);
 
-    const int row_tiles = A.inter >> 3, group = wave / SHARE;
-    const int first_tile = (unit * A.tiles * (W / SHARE)) + group, step_tiles = W / SHARE;   // this wave's: first_tile + step_tiles i
-    const int my_tiles = first_tile >= row_tiles ? 0 : std::min((row_tiles - first_tile + step_tiles - 1) / step_tiles, A.tiles);
+    const int row_tiles = (A.inter + 15) >> 4;
+    constexpr int AT_ONCE = W / SHARE;                       // tiles
+    const int local0 = wave / SHARE, tile0 = unit * A.tiles * AT_ONCE, first_tile = tile0 + local0;   // this wave's: first_tile + AT_ONCE i
+    const int my_tiles = first_tile >= row_tiles ? 0 : std::min((row_tiles - first_tile + AT_ONCE - 1) / AT_ONCE, A.tiles);
     const int k_begin = A.kb * (wave % SHARE) / SHARE, k_end = A.kb * (wave % SHARE + 1) / SHARE;
     const uint8_t * weights = A.w + static_cast<int64_t>(expert) * A.rows * A.k_bytes;
     uint8_t * mine = ring + wave * (D * S::STEP);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(mine));
 
-    // entries: the ones that this lane loads pieces of, and its column's
-    const int row_bytes = R::TERMS == 3 ? A.k_bytes / (one_byte(KIND) ? 1 : 2) * 4 : A.k_bytes / (one_byte(KIND) ? 1 : 2) * 2;
-    const uint8_t * rows[NB];
-    int piece[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int flat = 64 * i + lane, c = flat / R::PIECES, entry = list[wave][c < n ? c : 0];
-        rows[i] = static_cast<const uint8_t *>(A.x) + static_cast<int64_t>(entry / A.top_k) * row_bytes;
-        piece[i] = (flat % R::PIECES) ^ (c & 7);
-    }
+    const int row_bytes = A.k_bytes / (one_byte(KIND) ? 1 : 2) * (X == VBM_TYPE_F32 ? 4 : 2);
+    typename S::Source source;
+    S::enter(source, list[wave], n, [&](int entry) { return static_cast<const uint8_t *>(A.x) + static_cast<int64_t>(entry / A.top_k) * row_bytes; });
     const int column = r / R::TERMS < n ? r / R::TERMS : 0, term = r % R::TERMS;
 
-    int tile_next = 0, kb_next = k_begin, slot_next = 0;
-    const uint8_t * base = nullptr;
-    const uint32_t offset[2] = {static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(A.k_bytes), static_cast<uint32_t>(lane >> 3) * static_cast<uint32_t>(A.k_bytes)};
-    const float * scale = nullptr;
+    int tile_next = 0, kb_next = k_begin, place_next = 0;
     auto enter = [&](int i) __attribute__((always_inline)) {
-        const int i0 = (first_tile + step_tiles * i) * 8;
-        base = weights + static_cast<int64_t>(i0) * A.k_bytes;
-        if constexpr (S::F8) scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + ((i0 + (q >= 2 ? A.inter : 0)) >> 7)) * A.kb;
+        const int i0 = (first_tile + AT_ONCE * i) * 16;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) source.base[g] = weights + static_cast<int64_t>(i0 + g * A.inter) * A.k_bytes;
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {                        // (the last tile's rows past I read its last one)
+            const int row = 8 * l + (lane >> 3);
+            source.offset[l] = source.offset[2 + l] = static_cast<uint32_t>(i0 + row < A.inter ? row : A.inter - 1 - i0) * static_cast<uint32_t>(A.k_bytes);
+        }
+        if constexpr (S::F8) source.scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + ((i0 + (lane >= 32 ? A.inter : 0)) >> 7)) * A.kb;
     };
     auto issue = [&]() __attribute__((always_inline)) {
-        S::load(lds0 + slot_next * S::STEP, base, base + static_cast<int64_t>(A.inter) * A.k_bytes, offset, rows, piece, scale, kb_next, A.k_bytes, row_bytes);
-        slot_next = slot_next + 1 == D ? 0 : slot_next + 1;
-        if (kb_next + 1 < k_end) {
+        S::load(lds0 + place_next * S::STEP, source, kb_next, A.k_bytes, row_bytes);
+        place_next = place_next + 1 == D ? 0 : place_next + 1;
+        if (kb_next + 1 < k_end) {                           // (past the end the last step again, so that the waits' counts hold)
             ++kb_next;
         } else if (tile_next + 1 < my_tiles) {
             kb_next = k_begin;
@@ -375,57 +485,65 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
 #pragma unroll
         for (int i = 0; i < D; ++i) issue();
     }
-    for (int i = threadIdx.x; i < step_tiles * A.tiles * 16; i += W * 64) {
-        const int at = (unit * A.tiles * step_tiles + (i >> 4)) * 8 + (i & 7) + (i & 8 ? A.inter : 0);
-        const bool live = (unit * A.tiles * step_tiles + (i >> 4)) < row_tiles;
-        row_bias[i] = A.bias && live ? A.bias[static_cast<int64_t>(expert) * A.rows + at] : 0.0f;
-        if constexpr (kScaled) row_scale[i] = live ? A.ws[static_cast<int64_t>(expert) * A.rows + at] : 0.0f;
+    for (int i = threadIdx.x; i < AT_ONCE * A.tiles * 32; i += W * 64) {
+        const int value = (tile0 + (i >> 5)) * 16 + (i & 15), at = value + (i & 16 ? A.inter : 0);
+        row_bias[i] = A.bias && value < A.inter ? A.bias[static_cast<int64_t>(expert) * A.rows + at] : 0.0f;
+        if constexpr (kScaled) row_scale[i] = value < A.inter ? A.ws[static_cast<int64_t>(expert) * A.rows + at] : 0.0f;
     }
     __syncthreads();
 
-    // tile i's sums to h: lane (c, j) has value j of entry c
-    auto finish = [&](int i) __attribute__((always_inline)) {
-        const int c = lane >> 3, j = lane & 7, local = (group + step_tiles * i) * 16;
-        if (c >= n) return;
-        float gate = 0.0f, up = 0.0f;
+    // Tile i's sums to h, as their three terms: lane (q, first column of an entry) has four values.
+    auto finish = [&](int i, f32x4 gate, f32x4 up) __attribute__((always_inline)) {
+        gate = over_terms<R::TERMS>(gate);
+        up = over_terms<R::TERMS>(up);
+        const int local = (local0 + AT_ONCE * i) * 32 + 4 * q, first = (first_tile + AT_ONCE * i) * 16 + 4 * q;
+        if (term || r / R::TERMS >= n || first >= A.inter) return;
+        if constexpr (kScaled) gate *= *reinterpret_cast<const f32x4 *>(row_scale + local), up *= *reinterpret_cast<const f32x4 *>(row_scale + local + 16);
+        gate += *reinterpret_cast<const f32x4 *>(row_bias + local);
+        up += *reinterpret_cast<const f32x4 *>(row_bias + local + 16);
+        float v[4];
 #pragma unroll
-        for (int s = 0; s < SHARE; ++s)
+        for (int e = 0; e < 4; ++e) v[e] = glu_value(A.activation, gate[e], up[e], A.alpha, A.limit);
+        uint8_t * to = A.h + (static_cast<int64_t>(list[wave][column]) * A.h_kb + first / R::VALUES) * A.h_step + first % R::VALUES * 2;
 #pragma unroll
-            for (int t = R::TERMS - 1; t >= 0; --t) {
-                gate += sums[wave + s][(c * R::TERMS + t) * 16 + j];
-                up += sums[wave + s][(c * R::TERMS + t) * 16 + 8 + j];
-            }
-        if constexpr (kScaled) gate *= row_scale[local + j], up *= row_scale[local + 8 + j];
-        const float v = glu_value(A.activation, gate + row_bias[local + j], up + row_bias[local + 8 + j], A.alpha, A.limit);
-        // its three terms
-        const float v1 = without(v, 0xFFFF0000u), v2 = without(v1, 0xFFFF0000u);
-        const int at = (first_tile + step_tiles * i) * 8 + j, kb = at / R::VALUES;
-        uint16_t * to = reinterpret_cast<uint16_t *>(A.h + (static_cast<int64_t>(list[wave][c]) * A.h_kb + kb) * A.h_step) + at % R::VALUES;
-        to[0] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v) >> 16);
-        to[R::VALUES] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v1) >> 16);
-        to[2 * R::VALUES] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v2) >> 16);
+        for (int t = 0; t < 3; ++t) {
+            *reinterpret_cast<u32x2q *>(to + t * R::VALUES * 2) = u32x2q{upper_halves(v[0], v[1]), upper_halves(v[2], v[3])};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = without(v[e], 0xFFFF0000u);
+        }
     };
 
-    int slot = 0;
+    int place = 0;
     for (int i = 0; i < (SHARE == 1 ? my_tiles : 1); ++i) {
-        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
         if (streams) {
             for (int kb = k_begin; kb < k_end; ++kb) {
                 landed<(D - 1) * S::LOADS>();
-                acc = S::multiply(mine + slot * S::STEP, column, term, A.k_bytes - kb * 128 - 32 * q, acc);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
+                S::multiply(mine + place * S::STEP, column, term, kb, A.k_bytes, acc);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
                 issue();
-                slot = slot + 1 == D ? 0 : slot + 1;
+                place = place + 1 == D ? 0 : place + 1;
             }
         }
-        *reinterpret_cast<f32x4 *>(&sums[wave][r * 16 + 4 * q]) = acc;
-        if constexpr (SHARE == 1) finish(i);
+        if constexpr (SHARE == 1) {
+            finish(i, acc[0], acc[1]);
+        } else {
+            landed<0>();                                     // (the waves' sums take the ring's memory)
+            f32x4 * parts = reinterpret_cast<f32x4 *>(mine);
+            parts[lane] = acc[0];
+            parts[64 + lane] = acc[1];
+            __syncthreads();
+            if (wave % SHARE || !my_tiles) return;
+#pragma unroll
+            for (int w = 1; w < SHARE; ++w) {
+                const f32x4 * other = reinterpret_cast<const f32x4 *>(mine + w * (D * S::STEP));
+                acc[0] += other[lane];
+                acc[1] += other[64 + lane];
+            }
+            finish(0, acc[0], acc[1]);
+        }
     }
     landed<0>();                                             // no load may land after the workgroup has ended
-    if constexpr (SHARE > 1) {
-        __syncthreads();
-        if (wave % SHARE == 0 && my_tiles > 0) finish(0);
-    }
 }
 
 // ------------------------------------------------------------------------------- down and combine
@@ -433,17 +551,18 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
 // go to the entries' places in LDS, except for a slot that an earlier wave began: those are added up behind it, in the waves' order.
 template <int KIND, int NB>
 __global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
-    using S = Ring<KIND, kTerms, NB>;
+    using S = Ring<KIND, kTerms, NB, 1>;
     using R = Rows<KIND, kTerms>;
     constexpr int W = 8, D = NB <= 2 ? 4 : 3;              // (what fits in LDS)
     constexpr bool kScaled = KIND == VBM_TYPE_I8;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[W * D * S::STEP];
     __shared__ __attribute__((aligned(16))) float y[kMostEntries * 16], heads[W][R::MOST * 16];
     __shared__ int32_t ids[kMostEntries];
+    __shared__ float shares[kMostEntries];
     __shared__ int experts[kMostEntries], counts[kMostEntries], list[kMostEntries * R::MOST], head_slot[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int q = lane >> 4, r = lane & 15, n0 = static_cast<int>(blockIdx.x) * 16;
-    for (int i = threadIdx.x; i < A.entries; i += W * 64) ids[i] = A.ids[i];
+    if (static_cast<int>(threadIdx.x) < A.entries) ids[threadIdx.x] = A.ids[threadIdx.x], shares[threadIdx.x] = A.weights[threadIdx.x];
     __syncthreads();
     const Slots slots(ids, A.entries, A.n_expert, A.capacity);
     const int n_slots = slots.count();
@@ -456,28 +575,20 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
     const int row_bytes = A.kb * R::BYTES;
 
     int next = begin, slot_next = A.kb ? begin / A.kb : 0, kb_next = begin - slot_next * A.kb, place_next = 0;
-    const uint8_t * base = nullptr, * rows[NB];
-    int piece[NB];
-    uint32_t offset[2];
+    typename S::Source source;
 #pragma unroll
     for (int l = 0; l < 2; ++l) {
         const int n = n0 + 8 * l + (lane >> 3);
-        offset[l] = static_cast<uint32_t>((n < A.rows ? n : A.rows - 1) - n0) * static_cast<uint32_t>(A.k_bytes);
+        source.offset[l] = static_cast<uint32_t>((n < A.rows ? n : A.rows - 1) - n0) * static_cast<uint32_t>(A.k_bytes);
     }
-    const float * scale = nullptr;
     auto enter = [&](int s) __attribute__((always_inline)) {
-        const int expert = __builtin_amdgcn_readfirstlane(experts[s]), n = counts[s];
-        base = A.w + (static_cast<int64_t>(expert) * A.rows + n0) * A.k_bytes;
-        if constexpr (S::F8) scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + (n0 >> 7)) * A.kb;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int flat = 64 * i + lane, c = flat / R::PIECES, entry = list[s * A.capacity + (c < n ? c : 0)];
-            rows[i] = static_cast<const uint8_t *>(A.x) + static_cast<int64_t>(entry) * row_bytes;
-            piece[i] = (flat % R::PIECES) ^ (c & 7);
-        }
+        const int expert = __builtin_amdgcn_readfirstlane(experts[s]);
+        source.base[0] = A.w + (static_cast<int64_t>(expert) * A.rows + n0) * A.k_bytes;
+        if constexpr (S::F8) source.scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + (n0 >> 7)) * A.kb;
+        S::enter(source, list + s * A.capacity, counts[s], [&](int entry) { return static_cast<const uint8_t *>(A.x) + static_cast<int64_t>(entry) * row_bytes; });
     };
     auto issue = [&]() __attribute__((always_inline)) {
-        S::load(lds0 + place_next * S::STEP, base, base, offset, rows, piece, scale, kb_next, A.k_bytes, row_bytes);
+        S::load(lds0 + place_next * S::STEP, source, kb_next, A.k_bytes, row_bytes);
         place_next = place_next + 1 == D ? 0 : place_next + 1;
         if (next + 1 < end) {                                // (past the end the last step again, so that the waits' counts hold)
             ++next;
@@ -488,37 +599,50 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
         }
     };
     if (lane == 0) head_slot[wave] = -1;
+    const int first_slot = slot_next, first_kb = kb_next;
     if (begin < end) {
-        int s = slot_next, kb = kb_next, place = 0;
-        enter(s);
+        enter(first_slot);
 #pragma unroll
         for (int i = 0; i < D; ++i) issue();
+    }
+    // This thread's output is that of token mine_t and row mine_n: the first ranks' scales and biases are asked for here, so that
+    // nobody waits for them at the end.
+    constexpr int AHEAD = 8;
+    const int mine_t = static_cast<int>(threadIdx.x) >> 4, mine_n = n0 + (lane & 15);
+    const bool puts = mine_t < A.n_tokens && mine_n < A.rows;
+    auto row_at = [&](int k) {                               // of rank k's expert; -1: none
+        const int e = ids[mine_t * A.top_k + k];
+        return static_cast<unsigned>(e) < static_cast<unsigned>(A.n_expert) ? static_cast<int64_t>(e) * A.rows + mine_n : -1;
+    };
+    float scales[AHEAD], biases[AHEAD];
+    if (puts) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t at = k < A.top_k ? row_at(k) : -1;
+            scales[k] = kScaled && at >= 0 ? A.ws[at] : 1.0f;
+            biases[k] = A.bias && at >= 0 ? A.bias[at] : 0.0f;
+        }
+    }
+    if (begin < end) {
+        int s = first_slot, kb = first_kb, place = 0;
         const int column = r / 3, term = r % 3;
         bool head = kb > 0;
         int n = counts[s];
-        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
         for (int i = begin; i < end; ++i) {
             landed<(D - 1) * S::LOADS>();
-            acc = S::multiply(mine + place * S::STEP, column < n ? column : 0, term, A.k_bytes - kb * 128 - 32 * q, acc);
+            S::multiply(mine + place * S::STEP, column < n ? column : 0, term, kb, A.k_bytes, acc);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
             issue();
             place = place + 1 == D ? 0 : place + 1;
             if (++kb == A.kb || i + 1 == end) {
-                // an entry's three columns are neighbouring lanes
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float sum = acc[e];                // (a bit cast of the vector's element itself would take the first one's)
-                    const int v = __builtin_bit_cast(int, sum);
-                    const float v1 = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, 0x101, 0xF, 0xF, true));
-                    const float v2 = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, v, 0x102, 0xF, 0xF, true));
-                    acc[e] += v2 + v1;
-                }
+                acc[0] = over_terms<3>(acc[0]);
                 if (term == 0 && column < n) {
                     float * to = head ? &heads[wave][column * 16] : y + list[s * A.capacity + column] * 16;
-                    *reinterpret_cast<f32x4 *>(to + 4 * q) = acc;
+                    *reinterpret_cast<f32x4 *>(to + 4 * q) = acc[0];
                 }
                 if (head && lane == 0) head_slot[wave] = s;
-                acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                acc[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 head = false;
                 kb = 0;
                 if (i + 1 < end) n = counts[++s];
@@ -535,28 +659,27 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
         }
     }
     __syncthreads();
-    // output row n0 + i % 16 of token i / 16: the ranks in their order
-    for (int i = threadIdx.x; i < A.n_tokens * 16; i += W * 64) {
-        const int t = i >> 4, n = n0 + (i & 15);
-        if (n >= A.rows) continue;
-        float v = 0.0f;
-        for (int k = 0; k < A.top_k; ++k) {
-            const int entry = t * A.top_k + k, expert = ids[entry];
-            if (expert == -1) continue;
-            float e = __builtin_nanf("");
-            if (static_cast<unsigned>(expert) < static_cast<unsigned>(A.n_expert)) {
-                const int64_t at = static_cast<int64_t>(expert) * A.rows + n;
-                e = y[entry * 16 + (i & 15)];
-                if constexpr (kScaled) e *= A.ws[at];
-                if (A.bias) e += A.bias[at];
-            }
-            v += A.weights[entry] * e;
-        }
-        const int64_t at = static_cast<int64_t>(t) * A.rows + n;
-        if (A.out_type == VBM_TYPE_F32) static_cast<float *>(A.out)[at] = v;
-        else if (A.out_type == VBM_TYPE_BF16) static_cast<__bf16 *>(A.out)[at] = static_cast<__bf16>(v);
-        else static_cast<_Float16 *>(A.out)[at] = static_cast<_Float16>(v);
+    if (!puts) return;
+    float v = 0.0f;
+    auto add = [&](int k, float scale, float bias) __attribute__((always_inline)) {   // the ranks in their order
+        const int entry = mine_t * A.top_k + k, expert = ids[entry];
+        if (expert == -1) return;
+        float e = static_cast<unsigned>(expert) < static_cast<unsigned>(A.n_expert) ? y[entry * 16 + (lane & 15)] : __builtin_nanf("");
+        if constexpr (kScaled) e *= scale;
+        if (A.bias) e += bias;
+        v += shares[entry] * e;
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+        if (k < A.top_k) add(k, scales[k], biases[k]);
+    for (int k = AHEAD; k < A.top_k; ++k) {
+        const int64_t at = row_at(k);
+        add(k, kScaled && at >= 0 ? A.ws[at] : 1.0f, A.bias && at >= 0 ? A.bias[at] : 0.0f);
     }
+    const int64_t at = static_cast<int64_t>(mine_t) * A.rows + mine_n;
+    if (A.out_type == VBM_TYPE_F32) static_cast<float *>(A.out)[at] = v;
+    else if (A.out_type == VBM_TYPE_BF16) static_cast<__bf16 *>(A.out)[at] = static_cast<__bf16>(v);
+    else static_cast<_Float16 *>(A.out)[at] = static_cast<_Float16>(v);
 }
 
 struct FewCall {
@@ -626,17 +749,17 @@ FewCall few_call(const vbm_moe_few_desc * d, int64_t n_tokens) {
     return c;
 }
 
-// Shared depth for few tiles: four waves a tile until each of the 1024 that run at once has four of its own.
+// All workgroups at once, two a CU (2048 waves): four or two waves a tile where there are few, several tiles a wave where there are many.
 template <int KIND, int X>
 void launch_gate_up(const FewCall & c, hipStream_t stream) {
     using R = Rows<KIND, X>;
     FewArgs a = c.up;
     a.capacity = std::min(R::MOST, a.n_tokens);
-    const int64_t row_tiles = a.inter / 8;
+    const int64_t row_tiles = (a.inter + 15) / 16;
     const double tiles = c.expected * static_cast<double>(row_tiles);
     auto go = [&](auto nb_c, auto share_c) {
         constexpr int NB = decltype(nb_c)::value, SHARE = decltype(share_c)::value, AT_ONCE = 4 / SHARE;
-        a.tiles = SHARE == 1 ? static_cast<int>(std::max(1.0, std::min(8.0, tiles / 4096))) : 1;
+        a.tiles = SHARE == 1 ? static_cast<int>(std::max(1.0, std::min<double>(kMostTiles, std::ceil(tiles / 2048 - 0.25)))) : 1;
         a.row_units = static_cast<int>((row_tiles + AT_ONCE * a.tiles - 1) / (AT_ONCE * a.tiles));
         const int64_t blocks = c.slots * a.row_units;
         require(blocks < (int64_t{1} << 24), "too many outputs for one launch");
@@ -644,7 +767,8 @@ void launch_gate_up(const FewCall & c, hipStream_t stream) {
         check_hip(hipGetLastError(), "few tokens gate_up launch");
     };
     auto shape = [&](auto nb_c) {
-        if (tiles >= 4096) go(nb_c, std::integral_constant<int, 1>{});
+        if (tiles > 1024) go(nb_c, std::integral_constant<int, 1>{});
+        else if (tiles > 512) go(nb_c, std::integral_constant<int, 2>{});
         else go(nb_c, std::integral_constant<int, 4>{});
     };
     const int nb = R::loads(a.capacity);
