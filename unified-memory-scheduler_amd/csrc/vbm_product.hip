@@ -585,6 +585,8 @@ struct Work {
 // i % 8, so each XCD takes a contiguous run of the list (group by group, row tile by row tile): the token tiles that share a row
 // tile's weights, and the row tiles that share the tokens, then meet in one L2. A group's tiles share its columns evenly. `launched`: the
 // most token tiles that rows grouped in order can have; offsets out of order may count more, and have the first ones done.
+// STRIP: so many token tiles of a group at a time, so that a run's weights and tokens are about as many.
+template <int STRIP>
 __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int row_tiles, int launched, Work & w) {
     const int n_rows = static_cast<int>(A.n_rows), slot = static_cast<int>(blockIdx.x >> 3);
     auto columns = [&](int lo, int hi) { return hi > lo ? (hi - lo + 15) >> 4 : 0; };
@@ -620,9 +622,14 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
         });
         if (!tiles) return false;
     }
-    const int local = item - before * row_tiles;
-    w.row_tile = local / tiles;
-    const int tile = local - w.row_tile * tiles, share = (columns(lo, hi) + tiles - 1) / tiles;
+    int local = item - before * row_tiles, first_tile = 0, strip = tiles;
+    if (STRIP && tiles > STRIP) {
+        first_tile = local / (row_tiles * STRIP) * STRIP;
+        local -= first_tile * row_tiles;
+        strip = tiles - first_tile < STRIP ? tiles - first_tile : STRIP;
+    }
+    w.row_tile = local / strip;
+    const int tile = first_tile + local - w.row_tile * strip, share = (columns(lo, hi) + tiles - 1) / tiles;
     w.first = lo + tile * share * 16;
     w.live = hi - w.first < share * 16 ? hi - w.first : share * 16;
     return w.live > 0;
@@ -648,7 +655,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
     constexpr int STAGE_BYTES = LDS - BT * (KIND == kI8 ? 8 : 4);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
     Work work;
-    if (!find_work(A, ST * WT, row_tiles, launched, work)) return;
+    if (!find_work<KIND == kI8 ? 8 : 0>(A, ST * WT, row_tiles, launched, work)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int q = lane >> 4, r = lane & 15, wn = wave / WT, wt = wave % WT;
     const int n0 = work.row_tile * BN;
@@ -707,6 +714,17 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
             tsrc[i] = A.b + token_row(8 * eight + (lane >> 3)) * A.k_bytes + piece * 16;
             place[i] = BN * 128 + eight * 1024;
         }
+        const int nw = n0 + 16 * SN * wn;                    // the wave's first output
+        f32x4 bias[SN], row_scales[SN];
+        auto fetch_bias = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int s = 0; s < SN; ++s) {
+                bias[s] = row_values(A, A.bias, work.group, nw + 16 * s + 4 * q);
+                row_scales[s] = KIND == kI8 ? row_values(A, A.ws, work.group, nw + 16 * s + 4 * q) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        };
+        // (integers leave registers for them: asked for here, they are waited for with the first stage)
+        if constexpr (KIND == kI8) fetch_bias();
         f32x4 acc[SN][NT];
 #pragma unroll
         for (int s = 0; s < SN; ++s)
@@ -807,6 +825,15 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
                 }
                 if constexpr (is_f8(KIND)) factor = sw * scale_now;
                 // (left to itself the compiler sums a product right behind its matrix instruction and waits for it)
+                if constexpr (KIND == kI8) {
+                    if (read) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+                    for (int s = 0; s < SN; ++s) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+                        if (last && MORE) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 if constexpr (KIND == kF8) {
                     if (read) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);          // the next column's reads
 #pragma unroll
@@ -852,13 +879,7 @@ __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, 
         // straight from the registers (16 rows x 32 bytes a store) the stores of a 4096 x 4096 output took 6 us longer.
         constexpr int ROW = 16 * SN * 4 + 16;                // bytes of a token's outputs there
         static_assert(W * 16 * ROW <= STAGE_BYTES, "the stages' memory holds them");
-        const int nw = n0 + 16 * SN * wn;                    // the wave's first output
-        f32x4 bias[SN], row_scales[SN];
-#pragma unroll
-        for (int s = 0; s < SN; ++s) {
-            bias[s] = row_values(A, A.bias, work.group, nw + 16 * s + 4 * q);
-            row_scales[s] = KIND == kI8 ? row_values(A, A.ws, work.group, nw + 16 * s + 4 * q) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        if constexpr (KIND != kI8) fetch_bias();
         uint8_t * mine = lds + wave * 16 * ROW;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
