@@ -108,7 +108,7 @@ class Layer:
         err = np.abs(got - y)[~bad]
         b = b + (8 * 2.0 ** -24 * np.abs(y).max() * self.K if gi is None else 0)
         if err.size:
-            print(f"worst error / bound {np.max(err / np.maximum(b[~bad], 1e-300)):.3f}, relative {np.linalg.norm(err) / np.linalg.norm(y[~bad]):.2g}", flush=True)
+            print(f"worst error / bound {np.max(err / np.maximum(b[~bad], 1e-300)):.3f}", flush=True)
         assert (err <= b[~bad]).all(), np.argwhere(err > b[~bad])[:4]
         if out_type == F32 and err.size and np.abs(y[~bad]).max() > 0:
             # (errors of random signs add up as their root: no more than a handful of fp32 steps of the whole)
@@ -135,10 +135,10 @@ def test_layer_from_logits(gpu, kind, x_type, T, E, K, H, I, act, bias):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("T,E,K,H,I", [(1, 128, 8, 2048, 768), (3, 32, 4, 2880, 2880), (16, 12, 4, 1440, 2000), (8, 5, 5, 2064, 4096), (1, 4, 1, 64, 16384 + 16)])
+@pytest.mark.parametrize("T,E,K,H,I", [(1, 12, 8, 2048, 768), (3, 6, 4, 1440, 1456), (16, 12, 4, 720, 1008), (8, 5, 5, 528, 4096), (1, 4, 1, 64, 16384 + 16),
+                                         (16, 60, 8, 64, 1040), (16, 60, 8, 32, 3216)])
 def test_layer_sizes(gpu, kind, T, E, K, H, I):
     """Shared and unshared depths, several row tiles a wave, rows that end inside a step."""
-    E = min(E, 40)
     L = Layer(kind, E, H, I, min(K, E), 1, True, seed=H)
     L.check(T, BF16, logits=(L.rng.standard_normal((T, E)) * 2).astype(np.float32), out_type=BF16)
 

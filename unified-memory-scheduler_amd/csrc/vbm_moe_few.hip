@@ -268,11 +268,14 @@ __device__ __forceinline__ bf16x8 widened(const unsigned * w, bf16x8 & rest) {
     }
 }
 
-// The same in all lanes, which the compiler does not see everywhere.
+// The same in all lanes, which the compiler does not see everywhere. (A load needs five wait states behind a vector instruction that writes
+// its scalar base; the compiler does not count into the inline assembly of the loads.)
 __device__ __forceinline__ const uint8_t * uniform(const uint8_t * p) {
     const uint64_t v = reinterpret_cast<uint64_t>(p);
     const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
-    return reinterpret_cast<const uint8_t *>(static_cast<uint64_t>(hi) << 32 | lo);
+    uint64_t u = static_cast<uint64_t>(hi) << 32 | lo;
+    asm volatile("s_nop 4" : "+s"(u));
+    return reinterpret_cast<const uint8_t *>(u);
 }
 
 // What a wave streams: G times 16 weight rows x 128 bytes a step, the step's activations of up to 64 NB pieces, FP8 scales.
@@ -350,7 +353,8 @@ struct Ring {
         f32x4 sum[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) sum[g] = F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[g];
-        const unsigned mask0 = term >= 1 ? 0xFFFF0000u : 0u, mask1 = term == 2 ? 0xFFFF0000u : 0u;
+        // term t of a value is what its first 8 (t + 1) significant bits have over its first 8 t
+        const unsigned kept = term == 1 ? 0xFFFFFF00u : 0xFFFFFFFFu, gone = term == 0 ? 0u : (term == 1 ? 0xFFFF0000u : 0xFFFFFF00u);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             u32x4 b;
@@ -371,8 +375,9 @@ struct Ring {
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    v[i] = without(v[i], mask0);
-                    if constexpr (X == VBM_TYPE_F32) v[i] = without(v[i], mask1);
+                    const unsigned bits = __builtin_bit_cast(unsigned, static_cast<float>(v[i]));
+                    // (fp16 has two terms, and the second one is all the rest)
+                    v[i] = __builtin_bit_cast(float, X == VBM_TYPE_F32 ? bits & kept : bits) - __builtin_bit_cast(float, bits & gone);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) b[i] = upper_halves(v[2 * i], v[2 * i + 1]);
