@@ -283,9 +283,10 @@ template <int KIND, int X, int NB, int G>
 struct Ring {
     using R = Rows<KIND, X>;
     static constexpr bool F8 = KIND == VBM_TYPE_F8_E4M3;
-    // (LOADS: a step's at least. The waits count on these; a step with more entries has more of them, and then somewhat more than the
-    // oldest step is waited for. Loads for nobody instead, by one lane, took 10 ns a step of a CU, of 70.)
-    static constexpr int LOADS = 2 * G + 1 + (F8 ? 1 : 0), ACTIVATIONS = G * 2048, SCALES = ACTIVATIONS + NB * 1024, STEP = SCALES + (F8 ? 256 : 0);
+    // (FEWEST, MOST: a step's loads; how many depends on its slot's entries. As many for all steps, those for nobody by one lane, took the down
+    // launch of four tokens 37.5 us instead of 35.4. gate_up's waits count them as they are: on the fewest, and so for later steps too, sixteen tokens
+    // over integers took 119 us instead of 110; down's, where it makes 1 % the other way, on the fewest.)
+    static constexpr int FEWEST = 2 * G + 1 + (F8 ? 1 : 0), MOST = FEWEST + NB - 1, ACTIVATIONS = G * 2048, SCALES = ACTIVATIONS + NB * 1024, STEP = SCALES + (F8 ? 256 : 0);
     static constexpr int NJ = R::VALUES / 32;
 
     // What the lane loads: its rows of weights (offset from the groups' bases), the entry's row and the piece of each load of activations; `live` loads
@@ -313,7 +314,8 @@ struct Ring {
     // Places of the weights' 16-byte pieces as in the grouped products' rings: piece p of row r at place p ^ (r / 2 % 8) of
     // its 128 bytes. Activations: entry c's pieces behind each other, p at place p ^ (c % 8), so that the lanes' reads
     // of one piece of several entries spread over the banks.
-    static __device__ __forceinline__ void load(uint32_t at, const Source & s, int kb, int k_bytes, int row_bytes) {
+    // Returns the number of loads.
+    static __device__ __forceinline__ int load(uint32_t at, const Source & s, int kb, int k_bytes, int row_bytes) {
         const int lane = threadIdx.x & 63, even = (lane & 7) ^ (lane >> 4), odd = even ^ 4;
         const int64_t off = static_cast<int64_t>(kb) * 128;
         // (a piece past the row's end reads the step's first one: zeros take its place in the registers)
@@ -331,6 +333,7 @@ struct Ring {
             load_to_lds_16(s.rows[i] + (b < row_bytes ? b : kb * R::BYTES), at + ACTIVATIONS + i * 1024);
         }
         if constexpr (F8) load_to_lds_4(s.scale + kb, at + SCALES);
+        return FEWEST - 1 + s.live;
     }
 
     // The step in `stage` added to acc: lane (q, r) has rows 4q .. 4q + 3 of column r of each group. entry, term: this lane's column.
@@ -410,6 +413,32 @@ struct Ring {
     }
 };
 
+// The loads of the N newest steps.
+template <int N>
+struct Newest {
+    int loads[N] = {};
+    __device__ __forceinline__ void add(int n) {
+#pragma unroll
+        for (int i = N - 1; i > 0; --i) loads[i] = loads[i - 1];
+        loads[0] = n;
+    }
+    // All others have landed, and the wave's LDS reads are done. FEWEST, MOST: of a step.
+    template <int FEWEST, int MOST>
+    __device__ __forceinline__ void landed_before() const {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += loads[i];
+        wait<N * FEWEST, N * MOST>(n);
+    }
+    template <int LEAST, int MOST>
+    static __device__ __forceinline__ void wait(int n) {
+        if constexpr (LEAST < MOST) {
+            if (n > LEAST) return wait<LEAST + 1, MOST>(n);
+        }
+        landed<LEAST>();
+    }
+};
+
 // Lane (q, r) with an entry's first column: its terms' columns, which are the neighbouring lanes, added up.
 template <int TERMS>
 __device__ __forceinline__ f32x4 over_terms(f32x4 acc) {
@@ -463,6 +492,7 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
     const int column = r / R::TERMS < n ? r / R::TERMS : 0, term = r % R::TERMS;
 
     int tile_next = 0, kb_next = k_begin, place_next = 0;
+    Newest<D - 1> newest;
     auto enter = [&](int i) __attribute__((always_inline)) {
         const int i0 = (first_tile + AT_ONCE * i) * 16;
 #pragma unroll
@@ -475,7 +505,7 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
         if constexpr (S::F8) source.scale = A.ws + (static_cast<int64_t>(expert) * ((A.rows + 127) >> 7) + ((i0 + (lane >= 32 ? A.inter : 0)) >> 7)) * A.kb;
     };
     auto issue = [&]() __attribute__((always_inline)) {
-        S::load(lds0 + place_next * S::STEP, source, kb_next, A.k_bytes, row_bytes);
+        newest.add(S::load(lds0 + place_next * S::STEP, source, kb_next, A.k_bytes, row_bytes));
         place_next = place_next + 1 == D ? 0 : place_next + 1;
         if (kb_next + 1 < k_end) {                           // (past the end the last step again, so that the waits' counts hold)
             ++kb_next;
@@ -523,7 +553,7 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
         f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
         if (streams) {
             for (int kb = k_begin; kb < k_end; ++kb) {
-                landed<(D - 1) * S::LOADS>();
+                newest.template landed_before<S::FEWEST, S::MOST>();
                 S::multiply(mine + place * S::STEP, column, term, kb, A.k_bytes, acc);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
                 issue();
@@ -635,7 +665,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
         int n = counts[s];
         f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
         for (int i = begin; i < end; ++i) {
-            landed<(D - 1) * S::LOADS>();
+            landed<(D - 1) * S::FEWEST>();
             S::multiply(mine + place * S::STEP, column < n ? column : 0, term, kb, A.k_bytes, acc);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
             issue();
