@@ -44,7 +44,8 @@ def same(got, want):
 @pytest.mark.parametrize("type_id", TYPES)
 @pytest.mark.parametrize("rows,k,stride,offset", [(1, 16, None, 0), (1, 2880, None, 0), (5, 512, None, 0), (7, 528, None, 0), (3, 2048, 2064, 0), (37, 2064, 2069, 1),
                                                   (9, 4096, None, 0), (6, 4112, 4200, 8), (4, 8192, None, 0), (3, 8208, None, 0), (2, 16384, None, 0),
-                                                  (2, 16400, None, 0), (2, 65536, 65537, 3), (1000, 208, None, 0), (5000, 96, 97, 0)])
+                                                  (2, 16400, None, 0), (2, 65536, 65537, 3), (1000, 208, None, 0), (5000, 96, 97, 0),
+                                                  (513, 2304, None, 0), (700, 4400, 4401, 0)])
 def test_quantize(gpu, type_id, rows, k, stride, offset):
     rng = np.random.default_rng(rows * 7 + k)
     x = (rng.standard_normal((rows, k)) * np.exp2(rng.integers(-6, 6, (rows, 1)))).astype(np.float32)
