@@ -585,7 +585,8 @@ struct Work {
 // i % 8, so each XCD takes a contiguous run of the list (group by group, row tile by row tile): the token tiles that share a row
 // tile's weights, and the row tiles that share the tokens, then meet in one L2. A group's tiles share its columns evenly. `launched`: the
 // most token tiles that rows grouped in order can have; offsets out of order may count more, and have the first ones done.
-// STRIP: so many token tiles of a group at a time, so that a run's weights and tokens are about as many.
+// STRIP: so many token tiles of a group at a time, so that a run has about as many rows of weights as of tokens (of 4096 x 4096 outputs, 4 x 8
+// tiles instead of 2 x 16).
 template <int STRIP>
 __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int row_tiles, int launched, Work & w) {
     const int n_rows = static_cast<int>(A.n_rows), slot = static_cast<int>(blockIdx.x >> 3);
@@ -645,8 +646,11 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 // block, half of a matrix instruction's time), the LDS reads under them; the rest is the loads' issue: a wave stands still until
 // the address unit has taken its kilobyte (18 cycles each, 64 of them a step), and the waves of a workgroup ask for it together.
 // What was tried: all of a step's loads at once 1.78; four-wave workgroups of 256 x 128 84 us; items dealt to the XCDs in turn, not in
-// runs: the same here, 5 % slower for ragged groups. Grouped prefill is bound by the weights' stream and what a workgroup
-// does not overlap with it: one of them fits a CU, and its start (bounds, rows, first stages) and end cost about 8 us of some 40.
+// runs: the same here, 5 % slower for ragged groups. Integers 56.6 us, 2.4 POPS (a library's int8 product with int32 outputs takes 72): their matrix
+// instructions alone take 40 at the rate that random data leaves them, without the loads it is 53, without the LDS reads 56; token tiles in
+// strips of 8 save 0.6, a column's reads ahead of its products 1.9. The 32 x 32 x 32 instruction, with the same tiles, took 65. Grouped prefill is bound by the weights' stream and what a workgroup
+// does not overlap with it: one of them fits a CU, and its start (bounds, rows, first stages) and end cost about 8 us of some 40. (Integers, 1517
+// tokens top-8, 128 experts of 2048 x 768: 79 us, 60 of them without the stores; two workgroups a CU of 128 x 128 take 77 to 79 too.)
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
 __global__ __launch_bounds__(WN * WT * 64) void many_rows_kernel(ProductArgs A, int row_tiles, int launched) {
     constexpr int W = WN * WT, BN = 16 * SN * WN, BT = 16 * ST * WT;

@@ -17,7 +17,9 @@ namespace vbm {
 //        1536 x 2048 123 against 156. Up to 10 rows a group both take as long: one token through 8 experts 9.2 (7.1 against 6.6 with the
 //        weights in the caches), 64 tokens top-4 over 32 experts of 5760 x 2880 103 and 104. An fp16 output's rounding, 2e-4, would not cover it.
 //   kF16, kBF16: as they are.
-//   kI8: 8-bit integers, by the integer matrix instruction, at the FP8 one's rate: exact products and sums.
+//   kI8: 8-bit integers, by the integer matrix instruction: exact products and sums. On random data it reaches 3.4 POPS alone, the FP8 one 3.9 PFLOP/s
+//        (on zeros 4.4 to 4.9 both: the clock gives way to the power). The choices below are within 10 % of the best of the five shapes from 12 to
+//        8000 tokens x 2880 x 2880, 1536 x 4096 and 6144 x 1024, and from 12 to 512 rows a group of 16 to 128 experts.
 enum Kind { kF8Wide, kF8, kF16, kBF16, kI8 };
 constexpr bool is_f8(int kind) { return kind == kF8Wide || kind == kF8; }
 
