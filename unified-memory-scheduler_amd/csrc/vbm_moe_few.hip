@@ -11,7 +11,7 @@
 // are two bf16 values), and so are the activations, as sums of bf16 values: fp32 ones of three (8 + 8 + 8 bits, each the leading
 // bits of what is left, so the last one is exact), fp16 of two, bf16 of one. Each term is a column of the matrix instruction's B operand, whose
 // 16 columns a few tokens would leave unused anyway: 5 rows of three terms or 8 of one or two. All products are exact in fp32, as in an fp32
-// program, and summed in fp32; h is kept as its three terms. An infinity or NaN in x makes its token's outputs NaN.
+// program, and summed in fp32; h is kept as its three terms. (An infinity's second term is a NaN.)
 //
 // Rows are grouped by expert into slots of up to as many (token, rank) entries as there are columns, in the order in which they first
 // appear; every wave finds its slot by itself from the ids: with ten ballots each lane knows the entries of its entry's expert.
