@@ -327,7 +327,7 @@ vbm_status vbm_glu_quantize_i8(int activation, int x_type, const void * gate, co
  *   s = x + residual, rounded to x_type     v = s / sqrt(mean(s^2) + eps) * weight, in fp32
  * over rows of k values (a multiple of 16, at most 65536). x and residual are of x_type (F32, F16 or BF16), rows x_stride and
  * residual_stride elements apart. residual may be NULL (s = x). sum, if given, gets s, laid out as residual; it may be the
- * residual's own buffer, or x's where both strides agree. weight [k] fp32 or NULL (ones). y, if given, gets v rounded to y_type,
+ * residual's own buffer, or x's where both strides agree (a call with others is refused). weight [k] fp32 or NULL (ones). y, if given, gets v rounded to y_type,
  * [n_rows][k]. codes (16-byte aligned), if given, [n_rows][k] of code_type: VBM_TYPE_F8_E4M3 with scales [n_rows][ceil(k / 128)] as
  * vbm_quantize_fp8 makes them of v, or VBM_TYPE_I8 with scales [n_rows] as vbm_quantize_i8 does. At least one of y and codes; eps > 0. A
  * row whose sum of squares is no fp32 number (a NaN, an infinity, or values that large) comes out as NaN: y NaN, scales NaN and

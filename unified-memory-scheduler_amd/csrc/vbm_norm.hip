@@ -319,6 +319,8 @@ vbm_status vbm_add_rms_norm_quantize(int x_type, const void * x, int64_t x_strid
         if (residual) {
             require_rows(x_type, residual, residual_stride, n_rows, k, "residual");
             require(at(sum, type_size(x_type)), "sum must be aligned to its type");
+            // (each row is read before its sum is stored, but not before another row's is)
+            require(sum != x || x_stride == residual_stride || n_rows <= 1, "sum may be x's buffer only with the same stride");
         } else {
             require(!sum, "there is no sum without a residual");
         }
