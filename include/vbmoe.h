@@ -378,8 +378,10 @@ vbm_status vbm_grouped_mul_mat(const vbm_weights * w, const void * b, const floa
 /* A routed-expert layer for a few tokens (up to 16, and up to 128 (token, rank) pairs) over weights as they are stored, in two launches:
  *   out[t] = sum over ranks r of weights[t][r] * (down[e] act(gate_up[e] x[t] + its bias) + its bias),  e = ids[t][r]
  * in the ranks' order. The activations are not quantized: x is taken as it is, F8 and I8 weights times their scales, and everything between
- * is held in fp32 (all products exact in fp32, fp32 sums); only out is rounded to its type. So results are nearer to the formula than those of the
- * chain above, which rounds the activations to 8 bits twice. */
+ * is held in fp32 (all products exact in fp32, fp32 sums; bits of a value below 2^-133 are dropped); only out is rounded to its type. So results are
+ * nearer to the formula than those of the chain above, which rounds the activations to 8 bits twice. F8 codes are summed over 128 of k, and I8 ones over
+ * all of it, before they meet their scales; these sums have to be fp32 numbers (they are for |x| up to 2^112 and 2^121 / k), and so do the hidden
+ * values: where one leaves the range, outputs may be NaN. An expert's weights are read once for every 4 to 8 (token, rank) pairs of it. */
 typedef struct vbm_moe_few_desc {
     vbm_weights gate_up;           /* [n_experts][2 * I][H]: rows [0, I) gate, [I, 2 * I) up; with bias or not  */
     vbm_weights down;              /* [n_experts][H][I], of gate_up's type                      */

@@ -129,3 +129,22 @@ def test_infinities(gpu, kind, x_type, act):
     with np.errstate(all="ignore"):
         assert np.isnan(L.want(v[bad], ids[bad], weights[bad], F32)[0]).all()
     assert np.isnan(got[bad]).all()
+
+
+@pytest.mark.parametrize("kind,code,size", [(F8, 0x7E, 111), (I8, 127, 113)])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+def test_sums_of_codes_up_to_the_end_of_fp32(gpu, kind, code, size, x_type):
+    """The largest codes times tokens of 2^size, in sums of 128 just below 2^127, whose scale brings them back to 112 (e4m3's 448) or 127. Their sigmoid is 1 in
+    fp32, and sums of the hidden values' squares are exact."""
+    H, I, T = 128, 64, 3
+    gu, dn = np.full((1, 2 * I, H), code, np.uint8), np.full((1, H, I), 0x38 if kind == F8 else 1, np.uint8)
+    s1 = np.full((1, 1, 1) if kind == F8 else (1, 2 * I), 2.0 ** -120, np.float32)
+    s2 = np.ones((1, 1, 1) if kind == F8 else (1, H), np.float32)
+    d = [vb.DeviceBuffer.from_array(a) for a in (gu, s1, dn, s2)]
+    L = Layer.__new__(Layer)
+    L.H, L.I, L.K, L.E = H, I, 1, 1
+    L.desc = vb.MoeFewDesc(vb.Weights(kind, d[0].ptr, d[1].ptr, None, 1, 2 * I, H), vb.Weights(kind, d[2].ptr, d[3].ptr, None, 1, H, I), 1, 0, ALPHA, LIMIT)
+    raw, _ = R.store_as(x_type, np.full((T, H), 2.0 ** size))
+    got, _, _ = L.run(T, x_type, raw, ids=np.zeros((T, 1), np.int32), weights=np.ones((T, 1), np.float32))
+    gate = {F8: 448, I8: 127}[kind] * 128 * 2.0 ** (size - 120)
+    assert gate in (112, 127) and (got == I * gate * gate).all()
