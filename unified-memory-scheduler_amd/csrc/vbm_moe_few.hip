@@ -9,12 +9,14 @@
 //
 // The activations are not quantized. The weights are widened to bf16, exactly (e4m3 has 4 significant bits, 8-bit integers have 8; fp16's 11
 // are two bf16 values), and so are the activations, as sums of bf16 values: fp32 ones of three (8 + 8 + 8 bits, each the leading
-// bits of what is left, so the last one is exact), fp16 of two, bf16 of one. Each term is a column of the matrix instruction's B operand, whose
+// bits of what is left, so the last one is exact, but for bits below bf16's smallest value, 2^-133), fp16 of two, bf16 of one. Each term is a column of the matrix instruction's B operand, whose
 // 16 columns a few tokens would leave unused anyway: 5 rows of three terms or 8 of one or two. All products are exact in fp32, as in an fp32
-// program, and summed in fp32; h is kept as its three terms. (An infinity's second term is a NaN.)
+// program, and summed in fp32, FP8 blocks and integer rows before their scales; h is kept as its three terms. (An infinity's second term is a NaN.)
 //
 // Rows are grouped by expert into slots of up to as many (token, rank) entries as there are columns, in the order in which they first
-// appear; every wave finds its slot by itself from the ids: with ten ballots each lane knows the entries of its entry's expert.
+// appear; every wave finds its slot by itself from the ids: with two ballots for each of an id's ten bits a lane knows the entries of its entry's
+// expert. An expert with more entries than a slot holds has its weights read once for each slot: sixteen tokens all through four bf16 experts of 2880 x 2880
+// take 84 + 47 us, two slots an expert and four in the second launch; four such tokens, one slot, 31 + 21.
 // The weights stream as in the grouped products: 16 rows by 128 bytes a step, loaded straight to a ring in LDS of each wave, with the
 // activations of the step behind them (they come from the L2, and the waits count all loads alike).
 #include <algorithm>
@@ -458,7 +460,8 @@ __device__ __forceinline__ f32x4 over_terms(f32x4 acc) {
 // A row tile is 16 gate rows and the 16 up rows of the same values of h. SHARE waves share a tile's depth and join their sums through LDS; or
 // (SHARE 1) each wave takes `tiles` of its own, one after the other through its ring, without barriers.
 //
-// One token through eight of 128 FP8 experts of 2048 x 768 (25 MB): 11 us, 2 of them the routing, some 5 a launch and the first loads; 16 tokens, 30 bf16
+// One token through eight of 128 FP8 experts of 2048 x 768 (25 MB): 11 us, 2 of them the routing, some 5 a launch and the first loads (16 tokens, 84
+// experts: 56 us from logits, 49 with the routing given; every workgroup routes before its first load, also those past the last slot); 16 tokens, 30 bf16
 // experts of 2880 x 2880 touched: 166 us, 6.0 TB/s (reads alone reach 5.6 to 6); four tokens in fp32, 16 integer experts: 61 us, 4.4 TB/s, of which splitting
 // x into its terms takes 8 (bf16 tokens 53). 8 + 8 rows a tile took 86 there, and 168 for bf16; an even share of all tiles for 512
 // workgroups, split inside tiles, 61 and 179; rings of two steps with three workgroups a CU the same as of three with two.
@@ -588,8 +591,9 @@ __global__ __launch_bounds__(256) void few_gate_up_kernel(FewArgs A) {
 
 // ------------------------------------------------------------------------------- down and combine
 // One token as above: 8.5 us for 12.6 MB, of which all but the 2.5 of the stream are a launch, the ids, the first loads and the combine; 30 bf16 experts 98 us
-// (5.1 TB/s), 16 integer ones 35. H / 16 workgroups leave CUs idle (180 of 256 for 2880), but each reads at up to 12 bytes a cycle: 8, 12 or
-// 16 waves, with rings as deep as fit, take the same time.
+// (5.1 TB/s), 16 integer ones 35. H / 16 workgroups, one a CU, leave CUs idle (180 of 256 work for 2880, 128 for 2048), and each reads at up to 12 bytes a cycle: 8, 12 or
+// 16 waves, with rings as deep as fit, take the same time. From H = 4096 to 5120 the launch needs a second round: eight FP8 experts of 1536 values
+// 15.4 and 25.5 us, 56 of them 72 and 126.
 //
 // A workgroup takes 16 rows of the output for all slots; its waves share all their steps in contiguous runs, slot by slot. A wave's sums of a slot
 // go to the entries' places in LDS, except for a slot that an earlier wave began: those are added up behind it, in the waves' order.
@@ -729,8 +733,8 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs A) {
 struct FewCall {
     int kind, x_type;
     FewArgs up, down;              // of the two launches
-    int64_t slots;                 // at most, and expected
-    double expected;
+    int64_t slots;                 // at most
+    double expected;               // experts that are hit
     size_t h_at, bytes;            // of the workspace
 };
 
@@ -794,7 +798,10 @@ FewCall few_call(const vbm_moe_few_desc * d, int64_t n_tokens) {
 }
 
 // All workgroups at once, two a CU (2048 waves): four or two waves a tile where there are few (384 tiles, one token: 13 us either way, 16 unshared), several
-// tiles a wave where there are many (5076 tiles: 166 us by three, 174 by one; 2385: 63 by one, 69 by two).
+// tiles a wave where there are many, so that fewer workgroups route and start. 131 layers of 141 to 21674 tiles, all weights, H of 1024 to 4096, by
+// every choice: this one takes 3 % longer than the best on average, 16 % at most. us a layer by 1, 2, 3, 4 tiles a wave: 21674 tiles, FP8, H 1024: 471, 396, 377, 366 (4 are
+// taken); 10550, FP8, H 2048: 267, 245, 235, 237 (4); 5076, bf16, H 2880: 273, 282, 269, 296 (3); 9172, FP8, H 2880: 326, 311, 330, 352 (4); 4033,
+// integers, H 4096: 186, 197, 174, 193 (2). Waves a tile: 305 tiles of integers 24 by four, 27 by two, 34 by one; 1609 101, 81, 73; 508 42, 37, 40 (four).
 template <int KIND, int X>
 void launch_gate_up(const FewCall & c, hipStream_t stream) {
     using R = Rows<KIND, X>;

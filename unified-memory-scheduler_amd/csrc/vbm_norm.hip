@@ -12,8 +12,11 @@
 //
 // Bound by bandwidth: each value is read once and held in registers, eight a lane and up to eight such chunks, while the row's sum and
 // maximum are found (DPP inside a wave, one exchange through LDS between the waves of a row). 8192 rows of 4096 bf16: norm with sum, y and
-// e4m3 codes 59 us (5.15 TB/s, where a large copy reaches 5.1), integers 21 us (4.8); 1517 of 2880 fp16, norm and integers, 11.8 us (3.3); one row
-// 3.2 us, of which a launch is 2, the rest two loads and two exchanges one after the other. (Rows of more than 16384 values spill up to 72 bytes a lane.)
+// e4m3 codes 59 us (5.15 TB/s, where a large copy reaches 5.1), integers 21 us (4.8); GLU of 8192 x 2880 fp32 pairs to integers 41 us (5.2), of
+// bf16 pairs 29 (4.0); 1517 of 2880 fp16, norm and integers, 11.8 us (3.3); one row 3.2 us, of which a launch is 2, the rest three loads (x, the
+// residual, the weight) and two exchanges one after the other: a chunk's loads stand in branches on the alignment and are waited for there, the sum's
+// stores with them. Rows of more than 16384 values have up to eight chunks, whose loads so follow each other too, and spill up to 72 bytes a lane: 1024 of 32768 bf16, norm with
+// sum, y and integers, 72 us (4.2 TB/s), one 9.4.
 #include <type_traits>
 
 #include "vbm_device.hpp"

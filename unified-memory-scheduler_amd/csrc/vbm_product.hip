@@ -646,9 +646,10 @@ __device__ __forceinline__ bool find_work(const ProductArgs & A, int most, int r
 // block, half of a matrix instruction's time), the LDS reads under them; the rest is the loads' issue: a wave stands still until
 // the address unit has taken its kilobyte (18 cycles each, 64 of them a step), and the waves of a workgroup ask for it together.
 // What was tried: all of a step's loads at once 1.78; four-wave workgroups of 256 x 128 84 us; items dealt to the XCDs in turn, not in
-// runs: the same here, 5 % slower for ragged groups. Integers 56.6 us, 2.4 POPS (a library's int8 product with int32 outputs takes 72): their matrix
+// runs: the same here, 5 % slower for ragged groups. Integers 57 to 58 us, 2.4 POPS (a library's int8 product with int32 outputs takes 72): their matrix
 // instructions alone take 40 at the rate that random data leaves them, without the loads it is 53, without the LDS reads 56; token tiles in
-// strips of 8 save 0.6, a column's reads ahead of its products 1.9. The 32 x 32 x 32 instruction, with the same tiles, took 65. Grouped prefill is bound by the weights' stream and what a workgroup
+// strips of 8 save 0.6, a column's reads ahead of its products 1.9. The 4 that the loads and the 1 that the reads add leave most of what is over the
+// 40 unexplained. The 32 x 32 x 32 instruction, with the same tiles, took 65. Integers of 12, 40, 100, 333 and 512 tokens x 2880 x 2880: 8.0, 8.9, 9.8, 13.0 and 14.4 us. Grouped prefill is bound by the weights' stream and what a workgroup
 // does not overlap with it: one of them fits a CU, and its start (bounds, rows, first stages) and end cost about 8 us of some 40. (Integers, 1517
 // tokens top-8, 128 experts of 2048 x 768: 79 us, 60 of them without the stores; two workgroups a CU of 128 x 128 take 77 to 79 too.)
 template <int KIND, int SN, int ST, int WN, int WT, int LDS>
