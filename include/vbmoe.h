@@ -395,8 +395,9 @@ vbm_status vbm_moe_few_workspace(const vbm_moe_few_desc * desc, int64_t n_tokens
 /* x [n_tokens][H] of x_type (F32, F16 or BF16; 16-byte aligned) -> out [n_tokens][H] of out_type (F32, F16 or BF16; it may be x's buffer).
  * logits [n_tokens][n_experts] fp32: each token's top_k and the softmax over them, as vbm_router_topk_softmax chooses them; ids and weights
  * [n_tokens][top_k], where given, receive them. logits NULL: ids and weights are the routing. There an id of -1 adds nothing, any other outside
- * [0, n_experts) makes its token's outputs NaN, and an expert may be listed more than once. A NaN in x makes its token's outputs NaN; an infinity
- * makes them NaN or what the formula gives. No token's values reach another one's.
+ * [0, n_experts) makes its token's outputs NaN, and an expert may be listed more than once; a token whose ids are all -1 is not read and
+ * comes out as zeros. A NaN in any other token makes its outputs NaN; an infinity makes them NaN or what the formula gives. No token's values
+ * reach another one's.
  * `workspace`: 16-byte aligned device memory of the size above; it holds nothing between calls, and calls that share one must not overlap.
  * Can be captured. A call repeated on the same inputs gives the same bits. n_tokens = 0 does nothing. */
 vbm_status vbm_moe_few_forward(const vbm_moe_few_desc * desc, int x_type, const void * x, const float * logits, int32_t * ids, float * weights,
